@@ -132,6 +132,7 @@ int twg_memcpy_d2d(void* dst_dev, const void* src_dev, size_t nbytes, void* stre
 int twg_memset(void* dst_dev, int value, size_t nbytes, void* stream);
 int twg_host_alloc_pinned(void** ptr, size_t nbytes);
 int twg_host_free_pinned(void* ptr);
+int twg_host_is_pinned(const void* ptr, int* pinned);   /* host memory the device reads directly, whoever allocated it */
 /* Strided / broadcasting device copy of `itemsize`-byte elements (1, 2, 4, 8 or 16).
  * Replaces unary_kernel<UnaryOp::Copy> (csrc/ops/copy.cpp:123-134, unary.cpp:88).
  * desc operands: [0] = out, [1] = in. */
@@ -322,6 +323,92 @@ int twg_fused_cache_stats(int64_t* hits, int64_t* misses);
 /* Generated CUDA source of a program (ahead-of-time programs report the same text NVRTC would
  * be given); the pointer stays valid until twg_fused_release. */
 int twg_fused_source(const TwgFusedProgram* p, const char** source);
+
+/* ---- the passes of a transformer between its matrix products -----------------------------------
+ * No counterpart in the reference (its op list, README.md:106-166, ends with the pointwise ops).
+ * Tensors are float32, float16 or bfloat16 (TWG_DTYPE_F32 / _F16 / _BF16); arithmetic is float32 and a
+ * result is rounded once.  None of the calls allocates, synchronises or keeps anything between
+ * calls, so they may be captured into a graph.
+ *
+ * Rotation of queries and keys by their positions.  Frequency j of a head (0 <= j < rot_dim / 2)
+ * turns its pair of elements, (j, j + rot_dim / 2) or with `adjacent` (2 j, 2 j + 1), by
+ * positions[axis_of[j]][b][s] * inv_freq[j] radians; elements from rot_dim on pass unturned.  The
+ * angle is formed in float64.  One axis is the usual rotation; several serve images and video,
+ * whose time, height and width turn their own frequencies. */
+#define TWG_ROTARY_MAX_FREQS 256
+typedef struct TwgRotaryDesc {
+  int32_t dtype;                   /* TwgDtype of q, k, their outputs and gradients */
+  int32_t weight_dtype;            /* of the norms' weights and their gradients: `dtype` or TWG_DTYPE_F32 */
+  int32_t position_dtype;          /* TWG_DTYPE_I32 or _I64; any value, negative ones turn backwards */
+  int32_t freq_dtype;              /* TWG_DTYPE_F32 or _F64 */
+  int32_t head_dim;                /* 2..512 */
+  int32_t rot_dim;                 /* even, 2..head_dim */
+  int32_t axes;                    /* 1..8 */
+  int32_t adjacent;                /* non-zero: pairs are neighbours */
+  int32_t inverse;                 /* twg_rotary only, non-zero: turn by the negated angle (the gradient) */
+  float eps;                       /* of the norms */
+  int64_t batch, seq;              /* batch * seq < 2^31 */
+  int64_t heads[2];                /* of q and of k; 0: that tensor is absent and its pointers may be NULL */
+  int64_t in_strides[2][4];        /* elements: batch, seq, head, dim of q and k */
+  int64_t out_strides[2][4];       /* of what the call writes: q_out and k_out, or dq and dk */
+  int64_t grad_strides[2][4];      /* of dq_out and dk_out (twg_qk_norm_rotary_backward) */
+  int64_t position_strides[3];     /* axis, batch, seq */
+  uint8_t axis_of[TWG_ROTARY_MAX_FREQS];  /* < axes for each of the rot_dim / 2 frequencies */
+} TwgRotaryDesc;
+/* An output may be its input itself (same pointer and strides); any other overlap is not allowed. */
+int twg_rotary(const TwgRotaryDesc* d, const void* q, const void* k, const void* positions, const void* inv_freq,
+               void* q_out, void* k_out, void* stream);
+/* The same with every head divided by the root of its mean square (+ eps) and multiplied by a weight
+ * of head_dim elements before it is turned, in the same pass.  A NULL weight counts as ones. */
+int twg_qk_norm_rotary(const TwgRotaryDesc* d, const void* q, const void* k, const void* q_weight, const void* k_weight,
+                       const void* positions, const void* inv_freq, void* q_out, void* k_out, void* stream);
+/* Its gradient, from the inputs of the forward call and the gradients dq_out, dk_out of what it wrote.
+ * dq_weight / dk_weight may be NULL.  The workspace (16-byte aligned) holds partial sums of the weights'
+ * gradients, is written before it is read, and may be NULL when both are; the sums are added in a
+ * fixed order.  The size depends on the descriptor alone; 0: the descriptor is not valid. */
+size_t twg_qk_norm_rotary_workspace_bytes(const TwgRotaryDesc* d);
+int twg_qk_norm_rotary_backward(const TwgRotaryDesc* d, const void* q, const void* k, const void* q_weight, const void* k_weight,
+                                const void* positions, const void* inv_freq, const void* dq_out, const void* dk_out, void* dq,
+                                void* dk, void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+/* Dropout whose mask is a function of (seed, offset, element) and is never stored:
+ * out = keep ? x / (1 - p) : 0, plus residual where that is not NULL.  desc operands: [0]=out, [1]=x,
+ * [2]=residual (only with one); element i is the i-th in the descriptor's order (dimension 0 fastest),
+ * whatever the strides, and is kept where word i % 4 of Philox4x32-10 with key `seed` and counter
+ * (i / 4, offset) is at least round(p 2^32).  The gradient is the same call on the gradient, without
+ * the residual.  state, if not NULL, points at two uint64 on the device, {seed, offset}, read by the
+ * kernel in place of `seed` and added to `offset`: a captured graph draws another mask in every
+ * replay by updating them.  0 <= p <= 1; p = 1 drops everything.  out may be x or residual itself. */
+int twg_dropout(const TwgIterDesc* desc, int dtype, const void* x, const void* residual, void* out, double p,
+                uint64_t seed, uint64_t offset, const uint64_t* state, void* stream);
+
+/* Log probabilities of given tokens under softmax(scale * logits), row by row, with each row's entropy
+ * and log normaliser (natural logarithms) and its `top` most probable tokens in falling order (equal
+ * logits: the lower index first; NaN counts as largest).  Outputs are dense: logp [rows][tokens_per_row],
+ * entropy and lse [rows], top_logp and top_ids [rows][top] (NULL when top is 0).
+ * -inf logits have no probability; a row of nothing else has logp = lse = -inf, entropy 0 and no
+ * gradient.  A NaN or +inf logit makes its row's numbers NaN.  A negative token is padding: logp 0, no
+ * gradient.  A token of vocab or more reads nothing: logp NaN, no gradient. */
+#define TWG_LOGPROBS_MAX_TOKENS 1024
+typedef struct TwgLogprobsDesc {
+  int32_t dtype;              /* TwgDtype of logits and dlogits */
+  int32_t token_dtype;        /* TWG_DTYPE_I32 or _I64 */
+  int32_t tokens_per_row;     /* 0..TWG_LOGPROBS_MAX_TOKENS */
+  int32_t top;                /* 0..32, at most vocab */
+  int64_t rows;               /* at most 2^27 */
+  int64_t vocab;              /* 1..2^30 */
+  int64_t row_stride;         /* elements from one row of logits to the next; a row is contiguous */
+  int64_t token_strides[2];   /* elements: row, token */
+  float scale;                /* the inverse temperature, > 0 */
+} TwgLogprobsDesc;
+int twg_token_logprobs(const TwgLogprobsDesc* d, const void* logits, const void* tokens, float* logp, float* entropy,
+                       float* lse, float* top_logp, int64_t* top_ids, void* stream);
+/* Gradient of logp, entropy and lse (any of dlogp, dentropy, dlse may be NULL; dense, shaped like the
+ * outputs) from the forward call's inputs and its entropy and lse.  dlogits must not overlap logits. */
+int twg_token_logprobs_backward(const TwgLogprobsDesc* d, const void* logits, const void* tokens, const float* entropy,
+                                const float* lse, const float* dlogp, const float* dentropy, const float* dlse,
+                                void* dlogits, int64_t dlogits_row_stride, void* stream);
 
 /* ---- the count exchange of the batch-sharded path ---------------------------------------------
  * No counterpart in the reference: it drives one device (`webgpu_device_count = 1`,

@@ -48,5 +48,7 @@ PYBIND11_MODULE(_C, m) {
   m.def("last_launch_path", []() { return twg_last_launch_path(); });
   m.def("set_nvrtc_path", [](const std::string& p) { TWG_TORCH_CHECK(twg_fused_set_nvrtc_path(p.c_str())); });
   m.def("masked_select_set_poll_budget", [](int64_t polls) { TWG_TORCH_CHECK(twg_masked_select_set_poll_budget(polls)); });
+  m.def("set_rng_state", &core::set_rng_state);
+  m.def("get_rng_state", &core::get_rng_state);
   m.def("version", []() { return std::string(twg_version()); });
 }

@@ -3,6 +3,7 @@
 // tensor, "not really caching, yet") and csrc/core/webgpu_device_guard.{h,cpp} (one device, one
 // default stream) with thin shims over the library's stream-ordered caching allocator, its
 // per-device stream pool and CUDA events.
+#include <ATen/detail/PrivateUse1HooksInterface.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <c10/macros/Macros.h>
 
@@ -186,6 +187,38 @@ struct WebGPUGuardImpl final : public c10::impl::DeviceGuardImplInterface {
 };
 
 C10_REGISTER_GUARD_IMPL(PrivateUse1, WebGPUGuardImpl);
+
+// What autograd's engine asks a backend for before it runs a backward pass on its device.
+struct WebGPUHooks final : public at::PrivateUse1HooksInterface {
+  static c10::DeviceIndex count() {
+    int n = 0;
+    return twg_device_count(&n) == TWG_OK ? static_cast<c10::DeviceIndex>(n) : 0;
+  }
+  bool isBuilt() const override { return true; }
+  bool isAvailable() const override { return count() > 0; }
+  bool hasPrimaryContext(c10::DeviceIndex index) const override { return index >= 0 && index < count(); }
+  c10::DeviceIndex deviceCount() const override { return count(); }
+  bool isPinnedPtr(const void* data) const override {
+    int pinned = 0;
+    return twg_host_is_pinned(data, &pinned) == TWG_OK && pinned != 0;
+  }
+  c10::DeviceIndex getCurrentDevice() const override { return current_device(); }
+  void setCurrentDevice(c10::DeviceIndex index) const override { set_current_device(index); }
+  c10::DeviceIndex exchangeDevice(c10::DeviceIndex index) const override {
+    const c10::DeviceIndex old = current_device();
+    if (index != old) set_current_device(index);
+    return old;
+  }
+  c10::DeviceIndex maybeExchangeDevice(c10::DeviceIndex index) const override {
+    return index < 0 ? current_device() : exchangeDevice(index);
+  }
+};
+
+static const bool hooks_registered = [] {
+  static WebGPUHooks hooks;
+  at::RegisterPrivateUse1HooksInterface(&hooks);
+  return true;
+}();
 
 }  // namespace core
 }  // namespace torch_webgpu

@@ -33,6 +33,10 @@ void* stream_handle(c10::DeviceIndex device, int index);
 
 c10::Allocator* getWebGPUCachingAllocator();
 
+// Seed and running offset behind aten::dropout (transformer.cpp).
+void set_rng_state(uint64_t seed, uint64_t offset);
+std::pair<uint64_t, uint64_t> get_rng_state();
+
 struct DeviceScope {
   c10::DeviceIndex prev;
   // Always re-asserts the CUDA current device: other libraries in the process (torch.cuda) may

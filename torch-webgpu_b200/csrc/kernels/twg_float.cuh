@@ -1,0 +1,82 @@
+// Element access for the kernels that read and write float32, float16 or bfloat16 and compute in
+// float32: 16-byte vectors of any of the three, and single elements.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "twg_launch.cuh"
+
+namespace twg {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// The one rounding of a result: to nearest, ties to even.
+template <class T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Elements of T in one 16-byte vector.
+template <class T> constexpr int kVecOf = 16 / (int)sizeof(T);
+
+__device__ __forceinline__ void unpack(const uint4& r, float (&f)[4], const float*) {
+  f[0] = as_f(r.x); f[1] = as_f(r.y); f[2] = as_f(r.z); f[3] = as_f(r.w);
+}
+__device__ __forceinline__ void unpack(const uint4& r, float (&f)[8], const __half*) {
+  const u32 w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __half2 h;
+    *reinterpret_cast<u32*>(&h) = w[i];
+    const float2 v = __half22float2(h);
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+__device__ __forceinline__ void unpack(const uint4& r, float (&f)[8], const __nv_bfloat16*) {
+  const u32 w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = as_f(w[i] << 16);
+    f[2 * i + 1] = as_f(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[4], const float*) {
+  return make_uint4(as_u(f[0]), as_u(f[1]), as_u(f[2]), as_u(f[3]));
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], const __half*) {
+  u32 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    w[i] = *reinterpret_cast<const u32*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], const __nv_bfloat16*) {
+  u32 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    w[i] = *reinterpret_cast<const u32*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Host side: bytes of a floating element type this family of kernels takes, 0 for any other.
+inline int float_size(int dtype) {
+  return dtype == TWG_DTYPE_F32 ? 4 : (dtype == TWG_DTYPE_F16 || dtype == TWG_DTYPE_BF16) ? 2 : 0;
+}
+
+// Call `fn` with a null pointer of the element type behind `dtype` (one of the three).
+template <class Fn>
+int dispatch_float(int dtype, Fn&& fn) {
+  if (dtype == TWG_DTYPE_F32) return fn(static_cast<float*>(nullptr));
+  if (dtype == TWG_DTYPE_F16) return fn(static_cast<__half*>(nullptr));
+  return fn(static_cast<__nv_bfloat16*>(nullptr));
+}
+
+}  // namespace twg

@@ -11,7 +11,7 @@ the result; they exist so that parity tests and small scripts can drive the C AB
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, byref, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, byref, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 
 import numpy as np
@@ -57,6 +57,47 @@ class FusedInstr(ctypes.Structure):
     _fields_ = [("opcode", c_int32), ("a", c_int32), ("b", c_int32), ("imm", c_float)]
 
 
+ROTARY_MAX_FREQS = 256
+LOGPROBS_MAX_TOKENS = 1024
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32),
+        ("weight_dtype", c_int32),
+        ("position_dtype", c_int32),
+        ("freq_dtype", c_int32),
+        ("head_dim", c_int32),
+        ("rot_dim", c_int32),
+        ("axes", c_int32),
+        ("adjacent", c_int32),
+        ("inverse", c_int32),
+        ("eps", c_float),
+        ("batch", c_int64),
+        ("seq", c_int64),
+        ("heads", c_int64 * 2),
+        ("in_strides", (c_int64 * 4) * 2),
+        ("out_strides", (c_int64 * 4) * 2),
+        ("grad_strides", (c_int64 * 4) * 2),
+        ("position_strides", c_int64 * 3),
+        ("axis_of", ctypes.c_uint8 * ROTARY_MAX_FREQS),
+    ]
+
+
+class LogprobsDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32),
+        ("token_dtype", c_int32),
+        ("tokens_per_row", c_int32),
+        ("top", c_int32),
+        ("rows", c_int64),
+        ("vocab", c_int64),
+        ("row_stride", c_int64),
+        ("token_strides", c_int64 * 2),
+        ("scale", c_float),
+    ]
+
+
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libtwg.so"
 _lib = None
 
@@ -97,6 +138,7 @@ SIGNATURES = {
     "twg_memset": (c_int, [c_void_p, c_int, c_size_t, c_void_p]),
     "twg_host_alloc_pinned": (c_int, [POINTER(c_void_p), c_size_t]),
     "twg_host_free_pinned": (c_int, [c_void_p]),
+    "twg_host_is_pinned": (c_int, [c_void_p, POINTER(c_int)]),
     "twg_copy_strided": (c_int, [POINTER(IterDesc), c_int, c_void_p, c_void_p, c_void_p]),
     "twg_fill": (c_int, [POINTER(IterDesc), c_int, ctypes.c_uint64, c_void_p, c_void_p]),
     "twg_unary_f32": (c_int, [c_int, POINTER(IterDesc), c_void_p, c_void_p, c_void_p]),
@@ -131,6 +173,13 @@ SIGNATURES = {
     "twg_fused_source": (c_int, [c_void_p, POINTER(c_char_p)]),
     "twg_fused_set_cache_dir": (c_int, [c_char_p]),
     "twg_fused_cache_stats": (c_int, [POINTER(c_int64), POINTER(c_int64)]),
+    "twg_rotary": (c_int, [POINTER(RotaryDesc)] + [c_void_p] * 7),
+    "twg_qk_norm_rotary": (c_int, [POINTER(RotaryDesc)] + [c_void_p] * 9),
+    "twg_qk_norm_rotary_workspace_bytes": (c_size_t, [POINTER(RotaryDesc)]),
+    "twg_qk_norm_rotary_backward": (c_int, [POINTER(RotaryDesc)] + [c_void_p] * 13 + [c_size_t, c_void_p]),
+    "twg_dropout": (c_int, [POINTER(IterDesc), c_int, c_void_p, c_void_p, c_void_p, c_double, c_uint64, c_uint64, c_void_p, c_void_p]),
+    "twg_token_logprobs": (c_int, [POINTER(LogprobsDesc)] + [c_void_p] * 8),
+    "twg_token_logprobs_backward": (c_int, [POINTER(LogprobsDesc)] + [c_void_p] * 8 + [c_int64, c_void_p]),
     "twg_comm_set_nccl_path": (c_int, [c_char_p]),
     "twg_comm_unique_id": (c_int, [c_void_p]),
     "twg_comm_init_rank": (c_int, [c_void_p, c_int, c_int, POINTER(c_void_p)]),
@@ -301,6 +350,44 @@ def make_desc(shape, operands) -> IterDesc:
                 d.strides[t][k] = 0
             else:
                 d.strides[t][k] = ostrides[dim - lead]
+    return d
+
+
+def rotary_desc(dtype: str, tokens, heads, head_dim: int, *, in_strides, out_strides, position_strides, grad_strides=None,
+                rot_dim: int | None = None, axes: int = 1, axis_of=None, adjacent: bool = False, inverse: bool = False,
+                eps: float = 1e-6, weight_dtype: str = "float32", position_dtype: str = "int64",
+                freq_dtype: str = "float32") -> RotaryDesc:
+    """Descriptor of twg_rotary and twg_qk_norm_rotary(_backward).
+
+    tokens is (batch, seq), heads (of q, of k; 0 for an absent one); in_strides, out_strides and
+    grad_strides hold the element strides (batch, seq, head, dim) of q's and of k's tensor; axis_of
+    names each frequency's axis (default: axis 0).  Types are names of DTYPES.
+    """
+    rot_dim = head_dim if rot_dim is None else rot_dim
+    d = RotaryDesc(DTYPES[dtype], DTYPES[weight_dtype], DTYPES[position_dtype], DTYPES[freq_dtype], head_dim, rot_dim, axes,
+                   int(adjacent), int(inverse), eps, tokens[0], tokens[1])
+    d.heads[:] = heads
+    for t in range(2):
+        d.in_strides[t][:] = in_strides[t]
+        d.out_strides[t][:] = out_strides[t]
+        if grad_strides is not None:
+            d.grad_strides[t][:] = grad_strides[t]
+    d.position_strides[:] = position_strides
+    if axis_of is not None:
+        if len(axis_of) != rot_dim // 2 or len(axis_of) > ROTARY_MAX_FREQS:
+            raise TwgError(TWG_ERR_INVALID, f"axis_of names {len(axis_of)} axes for {rot_dim // 2} frequencies")
+        if len(axis_of) and not 0 <= min(axis_of) <= max(axis_of) < axes:
+            raise TwgError(TWG_ERR_INVALID, f"axis_of must name axes 0..{axes - 1}")
+        ctypes.memmove(d.axis_of, bytes(axis_of), len(axis_of))
+    return d
+
+
+def logprobs_desc(dtype: str, rows: int, vocab: int, *, row_stride: int | None = None, tokens_per_row: int = 1, token_strides=None,
+                  top: int = 0, scale: float = 1.0, token_dtype: str = "int64") -> LogprobsDesc:
+    """Descriptor of twg_token_logprobs(_backward); tokens are dense [rows][tokens_per_row] by default."""
+    d = LogprobsDesc(DTYPES[dtype], DTYPES[token_dtype], tokens_per_row, top, rows, vocab, vocab if row_stride is None else row_stride)
+    d.token_strides[:] = (tokens_per_row, 1) if token_strides is None else token_strides
+    d.scale = scale
     return d
 
 

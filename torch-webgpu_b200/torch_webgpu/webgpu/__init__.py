@@ -17,6 +17,7 @@ __all__ = [
     "is_initialized", "is_available", "current_device", "device_count", "set_device", "device",
     "synchronize", "memory_stats", "memory_allocated", "memory_reserved", "max_memory_allocated",
     "reset_peak_memory_stats", "empty_cache", "current_stream_handle", "launch_count",
+    "manual_seed", "manual_seed_all", "initial_seed", "get_rng_state", "set_rng_state",
 ]
 
 
@@ -101,5 +102,26 @@ def launch_count() -> int:
     return _C.launch_count()
 
 
-def manual_seed_all(seed: int) -> None:  # the backend has no random ops; accepted for API parity
-    return None
+def manual_seed(seed: int) -> None:
+    """Seed dropout's generator and start over with its first offset."""
+    _C.set_rng_state(int(seed) % 2**64, 0)
+
+
+def manual_seed_all(seed: int) -> None:  # also called by torch.manual_seed
+    manual_seed(seed)
+
+
+def initial_seed() -> int:
+    return _C.get_rng_state()[0]
+
+
+def get_rng_state(device=None) -> torch.Tensor:
+    """Seed and offset of dropout's generator as 16 bytes on the host.  One generator serves all devices."""
+    return torch.tensor([v - 2**64 if v >= 2**63 else v for v in _C.get_rng_state()], dtype=torch.int64).view(torch.uint8)
+
+
+def set_rng_state(new_state: torch.Tensor, device=None) -> None:
+    state = new_state.cpu()
+    if state.dtype != torch.uint8 or state.shape != (16,):
+        raise ValueError("torch.webgpu.set_rng_state: not a state of get_rng_state")
+    _C.set_rng_state(*(v % 2**64 for v in state.clone().view(torch.int64).tolist()))

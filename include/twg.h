@@ -333,7 +333,7 @@ int twg_fused_source(const TwgFusedProgram* p, const char** source);
  * Rotation of queries and keys by their positions.  Frequency j of a head (0 <= j < rot_dim / 2)
  * turns its pair of elements, (j, j + rot_dim / 2) or with `adjacent` (2 j, 2 j + 1), by
  * positions[axis_of[j]][b][s] * inv_freq[j] radians; elements from rot_dim on pass unturned.  The
- * angle is formed in float64.  One axis is the usual rotation; several serve images and video,
+ * angle is formed in 64 bits.  One axis is the usual rotation; several serve images and video,
  * whose time, height and width turn their own frequencies. */
 #define TWG_ROTARY_MAX_FREQS 256
 typedef struct TwgRotaryDesc {
@@ -364,8 +364,8 @@ int twg_qk_norm_rotary(const TwgRotaryDesc* d, const void* q, const void* k, con
                        const void* positions, const void* inv_freq, void* q_out, void* k_out, void* stream);
 /* Its gradient, from the inputs of the forward call and the gradients dq_out, dk_out of what it wrote.
  * dq_weight / dk_weight may be NULL.  The workspace (16-byte aligned) holds partial sums of the weights'
- * gradients, is written before it is read, and may be NULL when both are; the sums are added in a
- * fixed order.  The size depends on the descriptor alone; 0: the descriptor is not valid. */
+ * gradients, which are added in a fixed order, and the tokens' cosines and sines; it is written before it
+ * is read.  Its size depends on the descriptor alone; 0: the descriptor is not valid. */
 size_t twg_qk_norm_rotary_workspace_bytes(const TwgRotaryDesc* d);
 int twg_qk_norm_rotary_backward(const TwgRotaryDesc* d, const void* q, const void* k, const void* q_weight, const void* k_weight,
                                 const void* positions, const void* inv_freq, const void* dq_out, const void* dk_out, void* dq,

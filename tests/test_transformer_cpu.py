@@ -80,10 +80,10 @@ def test_rotary_refusals(abi):
 def test_qk_norm_backward_refusals_and_workspace(abi):
     L, d = abi.lib(), rotary(abi)
     need = L.twg_qk_norm_rotary_workspace_bytes(ctypes.byref(d))
-    assert need == 4 * 128 * (3 + 3)                       # three tokens: a CTA each for q and for k
+    assert need == 4 * 128 * (1 + 1) + 3 * 4 * 128         # one CTA's sums for q and for k, three tokens' tables
     big = rotary(abi)
     big.seq = 1 << 20
-    assert L.twg_qk_norm_rotary_workspace_bytes(ctypes.byref(big)) == 4 * 128 * 148 * 4
+    assert L.twg_qk_norm_rotary_workspace_bytes(ctypes.byref(big)) == 4 * 128 * 148 * 2 + (1 << 20) * 4 * 128
 
     def call(ptrs, bytes_=need, desc=d):
         return L.twg_qk_norm_rotary_backward(ctypes.byref(desc), *ptrs, bytes_, None)

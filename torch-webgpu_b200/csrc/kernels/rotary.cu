@@ -10,17 +10,20 @@
 // token.  A group of lanes owns a row, each lane two 16-byte vectors that hold both partners of
 // its pairs, so a row is in registers between its load and its store and the norm's sum is a few
 // shuffles.  The angle is the only part that needs more than 32 bits (a position of 10^6 leaves
-// 2^-4 of a turn in float32): it is formed and reduced to half turns in float64, once per token
-// and frequency, and its sine and cosine wait in shared memory for every head of the token.
+// 2^-4 of a turn in float32): it is formed in 64-bit fractions of a turn, once per token and
+// frequency, and its sine and cosine wait in shared memory for every head of the token.
 #include "twg_float.cuh"
 
 namespace twg {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotMaxTile = 16;        // tokens whose tables one CTA holds at a time
+constexpr int kRotWarps = kRotThreads / 32;
+constexpr int kRotRounds = 10;         // rows of a lane group in a warp's tile, where there are enough
+constexpr int kRotMaxTile = 16;        // tokens in such a tile
+constexpr int kRotTable = 512;         // entries of its tables
 constexpr int kRotMaxDim = 512;
 constexpr int kRotMaxAxes = 8;
-constexpr int kRotGradCtas = 148 * 4;  // CTAs of the gradient kernel: one row of weight partial sums each
+constexpr int kRotGradCtas = 148 * 2;  // CTAs of the gradient kernel: one row of weight partial sums each
 
 struct RotaryArgs {
   const void* x[2];  // q, k
@@ -34,10 +37,11 @@ struct RotaryArgs {
   const void* freq;
   u32 seq, tokens;
   int D, R, slots, lanes;  // lanes: lanes of a row's group (a power of two)
-  int tile;                // tokens per CTA (and round)
-  int head_span;           // heads per CTA (forward)
+  int tile, head_span, parts;  // forward: tokens and heads per warp, warps per token
+  int step[2];             // backward: heads of q and of k that one round of a warp's lane groups takes (a power of two)
   int ctas[2];             // CTAs that work on q and on k (backward)
   float* partial;          // backward: [ctas[0] + ctas[1]][D]
+  const float* table;      // backward: rotary_table_kernel's
   float eps;
   float sign;              // -1 rotates backwards
   bool pos64, freq64, w32, adjacent;
@@ -57,6 +61,17 @@ __device__ __forceinline__ void slot_elems(const RotaryArgs& a, int p, int V, in
   if (!a.adjacent && p * V < half) { *e0 = p * V; *e1 = p * V + half; }
   else { *e0 = 2 * p * V; *e1 = *e0 + V; }
 }
+// The elements of pair j of slot p: partners of one angle, or neighbours behind the turned part.
+__device__ __forceinline__ void pair_elems(const RotaryArgs& a, int p, int j, int V, int* ea, int* eb) {
+  if (a.adjacent) {
+    *ea = 2 * (p * V + j);
+    *eb = *ea + 1;
+  } else {
+    slot_elems(a, p, V, ea, eb);
+    *ea += j;
+    *eb += j;
+  }
+}
 
 __device__ __forceinline__ void token_place(const RotaryArgs& a, u32 tok, i64* b, i64* s) {
   const u32 q = tok / a.seq;
@@ -64,44 +79,33 @@ __device__ __forceinline__ void token_place(const RotaryArgs& a, u32 tok, i64* b
   *s = tok - q * a.seq;
 }
 
-// Sine and cosine of every frequency for `n` tokens from `tok0`; entries beyond the rotated part
-// are the identity.
-template <int V>
-__device__ __forceinline__ void fill_tables(const RotaryArgs& a, u32 tok0, int n, float* cosine, float* sine) {
-  const int row = a.slots * V;
-  for (int i = threadIdx.x; i < n * row; i += kRotThreads) {
-    const int t = i / row, f = i - t * row;
-    float c = 1.0f, s = 0.0f;
-    if (f < (a.R >> 1)) {
-      i64 b, q;
-      token_place(a, tok0 + (u32)t, &b, &q);
-      const i64 off = (i64)a.axis_of[f] * a.ps[0] + b * a.ps[1] + q * a.ps[2];
-      const double pos = a.pos64 ? (double)static_cast<const i64*>(a.pos)[off] : (double)static_cast<const int*>(a.pos)[off];
-      const double fr = a.freq64 ? static_cast<const double*>(a.freq)[f] : (double)static_cast<const float*>(a.freq)[f];
-      double turns = pos * fr * 0.15915494309189533577;  // 1 / (2 pi)
-      turns -= rint(turns);
-      sincospif((float)(2.0 * turns), &s, &c);
-      s *= a.sign;
-    }
-    const int at = t * row + spot<V>(f / V, f % V, a.slots);
-    cosine[at] = c;
-    sine[at] = s;
-  }
+// Sine and cosine of frequency f at a token; the identity behind the turned part.
+__device__ __forceinline__ void angle(const RotaryArgs& a, int f, i64 at_token, float* c, float* s) {
+  *c = 1.0f;
+  *s = 0.0f;
+  if (f >= (a.R >> 1)) return;
+  const i64 off = (i64)a.axis_of[f] * a.ps[0] + at_token;
+  const double pos = a.pos64 ? (double)static_cast<const i64*>(a.pos)[off] : (double)static_cast<const int*>(a.pos)[off];
+  const double fr = a.freq64 ? static_cast<const double*>(a.freq)[f] : (double)static_cast<const float*>(a.freq)[f];
+  double turns = pos * fr * 0.15915494309189533577;  // 1 / (2 pi)
+  turns -= rint(turns);
+  sincospif((float)(2.0 * turns), s, c);
+  *s *= a.sign;
 }
 
-// Weights of one tensor in slot order: vector 0 of every slot, then vector 1.
+// Weights of one tensor by pairs: of the first partners, then of the second ones.
 template <class T, int V>
 __device__ __forceinline__ void fill_weights(const RotaryArgs& a, int tensor, float* w) {
   const int row = a.slots * V;
-  for (int i = threadIdx.x; i < 2 * row; i += kRotThreads) {
-    const int second = i >= row, f = i - second * row, p = f / V, j = f % V;
+  for (int i = threadIdx.x; i < 2 * row; i += (int)blockDim.x) {
+    const int second = i >= row, f = i - second * row;
     int e[2];
-    slot_elems(a, p, V, &e[0], &e[1]);
-    const int el = e[second] + j;
+    pair_elems(a, f / V, f % V, V, &e[0], &e[1]);
+    const int el = e[second];
     float v = 1.0f;
     if (a.w[tensor] && el < a.D)
       v = a.w32 ? static_cast<const float*>(a.w[tensor])[el] : to_f32(static_cast<const T*>(a.w[tensor])[el]);
-    w[second * row + spot<V>(p, j, a.slots)] = v;
+    w[second * row + spot<V>(f / V, f % V, a.slots)] = v;
   }
 }
 
@@ -127,97 +131,187 @@ struct Raw<T, 1> {
   float a, b;
 };
 
-template <class T, int V>
-__device__ __forceinline__ void load_raw(Raw<T, V>& r, const T* row, i64 sd, int e0, int e1, int D, bool on) {
-  if constexpr (V == 1) {
-    r.a = on ? to_f32(row[e0 * sd]) : 0.0f;
-    r.b = on && e1 < D ? to_f32(row[e1 * sd]) : 0.0f;
+// The pairs of a lane's slot.
+template <class T, int V, bool ADJ>
+__device__ __forceinline__ void to_pairs(const Raw<T, V>& r, float (&a)[V], float (&b)[V]) {
+  if constexpr (V == 1) { a[0] = r.a; b[0] = r.b; }
+  else if constexpr (!ADJ) {
+    unpack(r.a, a, static_cast<const T*>(nullptr));
+    unpack(r.b, b, static_cast<const T*>(nullptr));
   } else {
-    r.a = r.b = make_uint4(0, 0, 0, 0);
-    if (on) {
-      r.a = ld_v4(row + e0);
-      r.b = ld_v4(row + e1);
-    }
-  }
-}
-template <class T, int V>
-__device__ __forceinline__ void to_floats(const Raw<T, V>& r, float (&u)[V], float (&v)[V]) {
-  if constexpr (V == 1) { u[0] = r.a; v[0] = r.b; }
-  else {
+    float u[V], v[V];
     unpack(r.a, u, static_cast<const T*>(nullptr));
     unpack(r.b, v, static_cast<const T*>(nullptr));
-  }
-}
-template <class T, int V>
-__device__ __forceinline__ void store_row(T* row, i64 sd, int e0, int e1, int D, bool on, const float (&u)[V], const float (&v)[V]) {
-  if (!on) return;
-  if constexpr (V == 1) {
-    row[e0 * sd] = from_f32<T>(u[0]);
-    if (e1 < D) row[e1 * sd] = from_f32<T>(v[0]);
-  } else {
-    st_v4(row + e0, pack(u, static_cast<const T*>(nullptr)));
-    st_v4(row + e1, pack(v, static_cast<const T*>(nullptr)));
-  }
-}
-
-template <int V, bool ADJ>
-__device__ __forceinline__ void rotate(float (&u)[V], float (&v)[V], const float (&c)[V], const float (&s)[V]) {
-  if constexpr (ADJ) {  // partners are neighbours within a vector
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) {
-      const float a = u[2 * j], b = u[2 * j + 1];
-      u[2 * j] = a * c[j] - b * s[j];
-      u[2 * j + 1] = b * c[j] + a * s[j];
-      const float d = v[2 * j], e = v[2 * j + 1];
-      v[2 * j] = d * c[V / 2 + j] - e * s[V / 2 + j];
-      v[2 * j + 1] = e * c[V / 2 + j] + d * s[V / 2 + j];
+      a[j] = u[2 * j]; b[j] = u[2 * j + 1];
+      a[V / 2 + j] = v[2 * j]; b[V / 2 + j] = v[2 * j + 1];
     }
+  }
+}
+template <class T, int V, bool ADJ>
+__device__ __forceinline__ void store_pairs(T* row, i64 sd, int e0, int e1, int D, bool on, const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) {
+    if (!on) return;
+    row[e0 * sd] = from_f32<T>(a[0]);
+    if (e1 < D) row[e1 * sd] = from_f32<T>(b[0]);
   } else {
+    uint4 x, y;
+    if constexpr (!ADJ) {
+      x = pack(a, static_cast<const T*>(nullptr));
+      y = pack(b, static_cast<const T*>(nullptr));
+    } else {
+      float u[V], v[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float a = u[j], b = v[j];
-      u[j] = a * c[j] - b * s[j];
-      v[j] = b * c[j] + a * s[j];
+      for (int j = 0; j < V / 2; ++j) {
+        u[2 * j] = a[j]; u[2 * j + 1] = b[j];
+        v[2 * j] = a[V / 2 + j]; v[2 * j + 1] = b[V / 2 + j];
+      }
+      x = pack(u, static_cast<const T*>(nullptr));
+      y = pack(v, static_cast<const T*>(nullptr));
+    }
+    if (on) {
+      st_v4(row + e0, x);
+      st_v4(row + e1, y);
     }
   }
 }
 
 __device__ __forceinline__ float group_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (lanes > 16) v += __shfl_xor_sync(0xffffffffu, v, 16);
+  if (lanes > 8) v += __shfl_xor_sync(0xffffffffu, v, 8);
+  if (lanes > 4) v += __shfl_xor_sync(0xffffffffu, v, 4);
+  if (lanes > 2) v += __shfl_xor_sync(0xffffffffu, v, 2);
+  if (lanes > 1) v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v;
 }
 
-// Forward: a CTA takes `tile` tokens and `head_span` of their q and k heads.
-template <class T, int V, int NS, bool NORM, bool ADJ>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
-  extern __shared__ __align__(16) float smem[];
-  __shared__ i64 offs[kRotMaxTile][4];  // token offsets of q, k, q_out, k_out
-  const int row = a.slots * V;
-  float* cosine = smem;
-  float* sine = cosine + a.tile * row;
-  float* w = sine + a.tile * row;  // NORM: q's weights, then k's
-  const int H = a.heads[0] + a.heads[1];
-  const int h0 = (int)blockIdx.y * a.head_span, span = min(a.head_span, H - h0);
-  const u32 tok0 = blockIdx.x * (u32)a.tile;
-  const int ntok = (int)min((u32)a.tile, a.tokens - tok0);
-  fill_tables<V>(a, tok0, ntok, cosine, sine);
-  if constexpr (NORM) {
-    fill_weights<T, V>(a, 0, w);
-    fill_weights<T, V>(a, 1, w + 2 * row);
-  }
-  if ((int)threadIdx.x < ntok) {
-    i64 b, s;
-    token_place(a, tok0 + threadIdx.x, &b, &s);
+// Arithmetic on neighbours j, j + 1 of a lane's arrays in one instruction, where both are in
+// registers side by side (V > 1).  The kernels issue three instructions for two of the copy's rate
+// in scalar form; V == 1 keeps that form.
+struct Two {
+  u64 v;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ void get(float& x, float& y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+};
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// A lane's V values as they are computed with: pairs of them, or the one.
+template <int V>
+struct Lanes {
+  static constexpr int N = V / 2;
+  Two x[N];
+  __device__ __forceinline__ void set(const float (&f)[V]) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      offs[threadIdx.x][t] = b * a.xs[t][0] + s * a.xs[t][1];
-      offs[threadIdx.x][2 + t] = b * a.ys[t][0] + s * a.ys[t][1];
+    for (int i = 0; i < N; ++i) x[i] = Two(f[2 * i], f[2 * i + 1]);
+  }
+  __device__ __forceinline__ void get(float (&f)[V]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i].get(f[2 * i], f[2 * i + 1]);
+  }
+  static __device__ __forceinline__ Two all(float f) { return Two(f, f); }
+  static __device__ __forceinline__ float sum(Two t) {
+    float a, b;
+    t.get(a, b);
+    return a + b;
+  }
+};
+template <>
+struct Lanes<1> {
+  static constexpr int N = 1;
+  float x[1];
+  __device__ __forceinline__ void set(const float (&f)[1]) { x[0] = f[0]; }
+  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = x[0]; }
+  static __device__ __forceinline__ float all(float f) { return f; }
+  static __device__ __forceinline__ float sum(float t) { return t; }
+};
+__device__ __forceinline__ float mul(float a, float b) { return a * b; }
+__device__ __forceinline__ float fma(float a, float b, float c) { return fmaf(a, b, c); }
+template <int V>
+using Wide = std::conditional_t<V == 1, float, Two>;
+
+// The two vectors (or elements) of a lane's slots in one row.  Without a row the registers keep what
+// they hold: a load costs no clearing, and nothing computed from them is stored.
+template <class T, int V, int NS>
+struct Row {
+  Raw<T, V> r[NS];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      if constexpr (V == 1) r[i].a = r[i].b = 0.0f;
+      else r[i].a = r[i].b = make_uint4(0, 0, 0, 0);
     }
   }
-  __syncthreads();
+  __device__ __forceinline__ void load(const T* row, i64 sd, const int (&e0)[NS], const int (&e1)[NS], const bool (&has)[NS], int D, bool on) {
+    if (!on) return;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      if (!has[i]) continue;
+      if constexpr (V == 1) {
+        r[i].a = to_f32(row[e0[i] * sd]);
+        if (e1[i] < D) r[i].b = to_f32(row[e1[i] * sd]);
+      } else {
+        r[i].a = ld_v4(row + e0[i]);
+        r[i].b = ld_v4(row + e1[i]);
+      }
+    }
+  }
+};
 
-  const int groups = kRotThreads / a.lanes, group = threadIdx.x / a.lanes, p0 = threadIdx.x & (a.lanes - 1);
-  const int items = ntok * span;
+// The row a lane group works on: token within the warp's tile and head within its span.
+struct Place {
+  int t, h;
+  __device__ __forceinline__ Place(int group, int span) : t(group / span), h(group - t * span) {}
+  __device__ __forceinline__ void advance(int groups, int span) {
+    h += groups;
+    while (h >= span) {
+      h -= span;
+      ++t;
+    }
+  }
+};
+
+// Forward: every warp works by itself on `tile` tokens and `head_span` of their q and k heads, about
+// kRotRounds rows to a lane group.  It issues the loads of its first rows, forms the tables while
+// they travel, and from then on always has the next rows on their way.  16384 tokens of 32 + 8 heads
+// of 128 in bfloat16 take 60.8 us (5.5 TB/s, 84 % of the copy bandwidth).  Measured and dropped: tables
+// of a CTA behind a barrier 63.9 us; no loop, one or two rows to a lane group 76 and 61 us (82 us where
+// the norm's weights add to what a CTA does first, 59.7 us here); the cosines of a token in registers
+// and rows two at a time 66 to 70 us; angles from 64-bit fractions of a turn instead of float64 65 us.
+template <class T, int V, int NS, bool NORM, bool ADJ>
+__global__ void __launch_bounds__(kRotThreads, V == 8 ? 5 : V > 1 ? 4 : 1) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  extern __shared__ __align__(16) float smem[];
+  __shared__ i64 all_offs[kRotWarps][kRotMaxTile][4];  // token offsets of q, k, q_out, k_out
+  const int row = a.slots * V, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* w = smem;  // NORM: q's weights, then k's
+  float* cosine = smem + (NORM ? 4 * row : 0) + warp * 2 * a.tile * row;
+  float* sine = cosine + a.tile * row;
+  auto& offs = all_offs[warp];
+  const u32 unit = blockIdx.x * kRotWarps + warp, tile = unit / (u32)a.parts;
+  const int h0 = (int)(unit - tile * (u32)a.parts) * a.head_span, span = min(a.head_span, a.heads[0] + a.heads[1] - h0);
+  const i64 tok0 = (i64)tile * a.tile;
+  const int ntok = (int)max((i64)0, min((i64)a.tile, (i64)a.tokens - tok0));
+  if (lane < ntok) {
+    i64 b, s;
+    token_place(a, (u32)tok0 + lane, &b, &s);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      offs[lane][t] = b * a.xs[t][0] + s * a.xs[t][1];
+      offs[lane][2 + t] = b * a.ys[t][0] + s * a.ys[t][1];
+    }
+  }
+  __syncwarp();
+
+  const int groups = 32 / a.lanes, p0 = lane & (a.lanes - 1);
   int e0[NS], e1[NS];
   bool has[NS];
 #pragma unroll
@@ -225,165 +319,270 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
     slot_elems(a, p0 + 32 * i, V, &e0[i], &e1[i]);
     has[i] = p0 + 32 * i < a.slots;
   }
-  Raw<T, V> cur[NS], nxt[NS];
-  auto fetch = [&](Raw<T, V>(&r)[NS], int item) {
-    const bool on = item < items;
-    const int t = on ? item / span : 0, h = h0 + (on ? item - t * span : 0);
-    const int z = h >= a.heads[0] ? 1 : 0;
-    const T* base = static_cast<const T*>(a.x[z]) + offs[t][z] + (i64)(h - (z ? a.heads[0] : 0)) * a.xs[z][2];
-#pragma unroll
-    for (int i = 0; i < NS; ++i) load_raw<T, V>(r[i], base, a.xs[z][3], e0[i], e1[i], a.D, on && has[i]);
+  Row<T, V, NS> x;
+  x.clear();
+  auto fetch = [&](const Place& at) {
+    const bool on = at.t < ntok;
+    const int h = h0 + at.h, z = h >= a.heads[0] ? 1 : 0;
+    x.load(static_cast<const T*>(a.x[z]) + (on ? offs[at.t][z] : 0) + (i64)(h - (z ? a.heads[0] : 0)) * a.xs[z][2], a.xs[z][3], e0, e1, has,
+           a.D, on);
   };
-  fetch(cur, group);
-  for (int first = 0; first < items; first += groups) {
-    const int item = first + group;
-    fetch(nxt, item + groups);
-    const bool on = item < items;
-    const int t = on ? item / span : 0, h = h0 + (on ? item - t * span : 0);
-    const int z = h >= a.heads[0] ? 1 : 0;
-    float u[NS][V], v[NS][V];
+  Place at(lane / a.lanes, span);
+  fetch(at);
+  for (int t = 0; t < ntok; ++t) {
+    i64 b, s;
+    token_place(a, (u32)tok0 + (u32)t, &b, &s);
+    for (int f = lane; f < row; f += 32) {
+      float c, sn;
+      angle(a, f, b * a.ps[1] + s * a.ps[2], &c, &sn);
+      cosine[t * row + spot<V>(f / V, f % V, a.slots)] = c;
+      sine[t * row + spot<V>(f / V, f % V, a.slots)] = sn;
+    }
+  }
+  if constexpr (NORM) {
+    fill_weights<T, V>(a, 0, w);
+    fill_weights<T, V>(a, 1, w + 2 * row);
+    __syncthreads();
+  } else {
+    __syncwarp();
+  }
+  const float inv_d = 1.0f / (float)a.D;
+  for (int left = ntok * span; left > 0; left -= groups) {
+    const bool on = at.t < ntok;
+    const int t = on ? at.t : 0, h = h0 + at.h, z = h >= a.heads[0] ? 1 : 0;
+    Lanes<V> u[NS], v[NS];
 #pragma unroll
-    for (int i = 0; i < NS; ++i) to_floats<T, V>(cur[i], u[i], v[i]);
+    for (int i = 0; i < NS; ++i) {
+      float f[V], g[V];
+      to_pairs<T, V, ADJ>(x.r[i], f, g);
+      u[i].set(f);
+      v[i].set(g);
+    }
+    at.advance(groups, span);
+    fetch(at);
     if constexpr (NORM) {
       float ss = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
+      for (int i = 0; i < NS; ++i) {
+        Wide<V> s0 = mul(u[i].x[0], u[i].x[0]), s1 = mul(v[i].x[0], v[i].x[0]);
 #pragma unroll
-        for (int j = 0; j < V; ++j) ss = fmaf(u[i][j], u[i][j], fmaf(v[i][j], v[i][j], ss));
-      const float r = rsqrtf(group_sum(ss, a.lanes) / (float)a.D + a.eps);
+        for (int j = 1; j < Lanes<V>::N; ++j) {
+          s0 = fma(u[i].x[j], u[i].x[j], s0);
+          s1 = fma(v[i].x[j], v[i].x[j], s1);
+        }
+        ss += Lanes<V>::sum(s0) + Lanes<V>::sum(s1);
+      }
+      const Wide<V> r = Lanes<V>::all(rsqrtf(fmaf(group_sum(ss, a.lanes), inv_d, a.eps)));
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        float w0[V], w1[V];
+        float f[V], g[V];
         const float* wz = w + z * 2 * row;
         const int p = has[i] ? p0 + 32 * i : 0;
-        read_row<V>(wz, p, a.slots, w0);
-        read_row<V>(wz + row, p, a.slots, w1);
+        read_row<V>(wz, p, a.slots, f);
+        read_row<V>(wz + row, p, a.slots, g);
+        Lanes<V> A, B;
+        A.set(f);
+        B.set(g);
 #pragma unroll
-        for (int j = 0; j < V; ++j) { u[i][j] *= r * w0[j]; v[i][j] *= r * w1[j]; }
+        for (int j = 0; j < Lanes<V>::N; ++j) {
+          u[i].x[j] = mul(u[i].x[j], mul(A.x[j], r));
+          v[i].x[j] = mul(v[i].x[j], mul(B.x[j], r));
+        }
       }
     }
     T* out = static_cast<T*>(a.y[z]) + offs[t][2 + z] + (i64)(h - (z ? a.heads[0] : 0)) * a.ys[z][2];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      float c[V], s[V];
+      float f[V], g[V];
       const int p = has[i] ? p0 + 32 * i : 0;
-      read_row<V>(cosine + t * row, p, a.slots, c);
-      read_row<V>(sine + t * row, p, a.slots, s);
-      rotate<V, ADJ>(u[i], v[i], c, s);
-      store_row<T, V>(out, a.ys[z][3], e0[i], e1[i], a.D, on && has[i], u[i], v[i]);
-      cur[i] = nxt[i];
+      read_row<V>(cosine + t * row, p, a.slots, f);
+      read_row<V>(sine + t * row, p, a.slots, g);
+      Lanes<V> C, S, A, B;
+      C.set(f);
+      S.set(g);
+#pragma unroll
+      for (int j = 0; j < Lanes<V>::N; ++j) {
+        A.x[j] = fma(u[i].x[j], C.x[j], mul(v[i].x[j], mul(S.x[j], Lanes<V>::all(-1.0f))));
+        B.x[j] = fma(v[i].x[j], C.x[j], mul(u[i].x[j], S.x[j]));
+      }
+      A.get(f);
+      B.get(g);
+      store_pairs<T, V, ADJ>(out, a.ys[z][3], e0[i], e1[i], a.D, on && has[i], f, g);
     }
   }
 }
 
+// Cosines and sines of the gradient's tokens: [tokens][2][slots V], quads of a slot as in shared memory.
+template <int V>
+__global__ void __launch_bounds__(kRotThreads) rotary_table_kernel(const __grid_constant__ RotaryArgs a, float* table) {
+  const int row = a.slots * V;
+  const i64 i = (i64)blockIdx.x * kRotThreads + threadIdx.x;
+  const u32 tok = (u32)(i / row);
+  const int f = (int)(i - (i64)tok * row);
+  if (tok >= a.tokens) return;
+  i64 b, s;
+  token_place(a, tok, &b, &s);
+  float c, sn;
+  angle(a, f, b * a.ps[1] + s * a.ps[2], &c, &sn);
+  float* to = table + (i64)tok * 2 * row + spot<V>(f / V, f % V, a.slots);
+  to[0] = c;
+  to[row] = sn;
+}
+
 // Gradient of norm and rotation.  With n = x r, r = rsqrt(mean(x^2) + eps), g = dy rotated back and
 // h = g w:  dx = r h - x r^3 mean(h x),  dw = sum over rows of g n.  Both sums over the head come
-// out of one round of shuffles.  A CTA walks token tiles of one tensor and keeps dw in registers
-// (a lane always owns the same elements); the CTAs' sums are added in a fixed order by
-// rotary_weight_grad_kernel, so the gradient does not depend on scheduling.
+// out of one round of shuffles.  A warp walks the tokens of one tensor, `tp` at a time, and their heads,
+// `hp` at a time: lane group g has token g / hp and head g % hp of them.  The next rows are always on
+// their way.  dw stays in registers (a lane always owns the same elements); the CTAs' sums are added
+// in a fixed order by rotary_weight_grad_kernel, so the gradient does not depend on scheduling.
+// The tables come from memory: formed here, between a warp's rows, they cost 40 of 140 us for 16384
+// tokens of 32 + 4 heads of 128.
 template <class T, int V, int NS, bool ADJ>
-__global__ void __launch_bounds__(kRotThreads) rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(kRotThreads, NS < 8 ? 2 : 1) rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
   extern __shared__ __align__(16) float smem[];
-  __shared__ i64 offs[kRotMaxTile][3];  // token offsets of x, dy, dx
-  const int row = a.slots * V;
-  float* cosine = smem;
-  float* sine = cosine + a.tile * row;
-  float* w = sine + a.tile * row;
-  float* red = w + 2 * row;  // [warps][2 * row]
-  const int z = (int)blockIdx.x >= a.ctas[0] ? 1 : 0;
-  const u32 mine = blockIdx.x - (z ? (u32)a.ctas[0] : 0u), stride = (u32)a.ctas[z] * (u32)a.tile;
-  const int H = a.heads[z];
+  const int row = a.slots * V, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* w = smem;
+  const int z = (int)blockIdx.x >= a.ctas[0] ? 1 : 0, H = a.heads[z];
   fill_weights<T, V>(a, z, w);
+  __syncthreads();
 
-  const int groups = kRotThreads / a.lanes, group = threadIdx.x / a.lanes, p0 = threadIdx.x & (a.lanes - 1);
+  const int group = lane / a.lanes, p0 = lane & (a.lanes - 1);
+  const int hp = a.step[z], tp = 32 / a.lanes / hp, tl = group / hp, hl = group & (hp - 1);
+  const i64 sx = a.xs[z][2] * hp, sg = a.gs[z][2] * hp, sy = a.ys[z][2] * hp;
+  const float inv_d = 1.0f / (float)a.D;
   int e0[NS], e1[NS];
   bool has[NS];
-  float dw0[NS][V], dw1[NS][V];
+  Lanes<V> dwa[NS], dwb[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
     slot_elems(a, p0 + 32 * i, V, &e0[i], &e1[i]);
     has[i] = p0 + 32 * i < a.slots;
 #pragma unroll
-    for (int j = 0; j < V; ++j) dw0[i][j] = dw1[i][j] = 0.0f;
+    for (int j = 0; j < Lanes<V>::N; ++j) dwa[i].x[j] = dwb[i].x[j] = Lanes<V>::all(0.0f);
   }
-  for (u32 tok0 = mine * (u32)a.tile; tok0 < a.tokens; tok0 += stride) {
-    const int ntok = (int)min((u32)a.tile, a.tokens - tok0);
-    __syncthreads();  // the previous round's tables are no longer read
-    fill_tables<V>(a, tok0, ntok, cosine, sine);
-    if ((int)threadIdx.x < ntok) {
-      i64 b, s;
-      token_place(a, tok0 + threadIdx.x, &b, &s);
-      offs[threadIdx.x][0] = b * a.xs[z][0] + s * a.xs[z][1];
-      offs[threadIdx.x][1] = b * a.gs[z][0] + s * a.gs[z][1];
-      offs[threadIdx.x][2] = b * a.ys[z][0] + s * a.ys[z][1];
+  // zero at first; later, where a group has no row, an earlier row of the same lanes and elements,
+  // which then counts times r = 0
+  Row<T, V, NS> xr, gr;
+  xr.clear();
+  gr.clear();
+  const u32 step = (u32)a.ctas[z] * kRotWarps * (u32)tp;
+  u32 tok = ((blockIdx.x - (z ? (u32)a.ctas[0] : 0u)) * kRotWarps + warp) * (u32)tp;  // first of the round's tokens
+  int h0 = 0;
+  const T *px = nullptr, *pg = nullptr;
+  T* py = nullptr;
+  const float* tab = nullptr;
+  auto place = [&] {  // addresses of this group's token
+    const u32 t = min(tok + (u32)tl, a.tokens - 1);
+    i64 b, s;
+    token_place(a, t, &b, &s);
+    px = static_cast<const T*>(a.x[z]) + b * a.xs[z][0] + s * a.xs[z][1] + hl * a.xs[z][2];
+    pg = static_cast<const T*>(a.g[z]) + b * a.gs[z][0] + s * a.gs[z][1] + hl * a.gs[z][2];
+    py = static_cast<T*>(a.y[z]) + b * a.ys[z][0] + s * a.ys[z][1] + hl * a.ys[z][2];
+    tab = a.table + (i64)t * 2 * row;
+  };
+  bool more = tok < a.tokens;
+  bool on = more && hl < H && tok + (u32)tl < a.tokens;
+  if (more) {
+    place();
+    xr.load(px, a.xs[z][3], e0, e1, has, a.D, on);
+    gr.load(pg, a.gs[z][3], e0, e1, has, a.D, on);
+  }
+  while (more) {
+    T* const out = py;
+    const float* const c_row = tab;
+    const bool now = on;
+    Lanes<V> xa[NS], xb[NS], ga[NS], gb[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      float f[V], g[V];
+      to_pairs<T, V, ADJ>(xr.r[i], f, g);
+      xa[i].set(f);
+      xb[i].set(g);
+      to_pairs<T, V, ADJ>(gr.r[i], f, g);
+      ga[i].set(f);
+      gb[i].set(g);
     }
-    __syncthreads();
-    const int items = ntok * H;
-    for (int first = 0; first < items; first += groups) {
-      const int item = first + group;
-      const bool on = item < items;
-      const int t = on ? item / H : 0;
-      const i64 h = on ? item - t * H : 0;
-      const T* xp = static_cast<const T*>(a.x[z]) + offs[t][0] + h * a.xs[z][2];
-      const T* gp = static_cast<const T*>(a.g[z]) + offs[t][1] + h * a.gs[z][2];
-      Raw<T, V> rx[NS], rg[NS];
+    // the next round: further heads, or the next tokens
+    h0 += hp;
+    if (h0 < H) {
+      px += sx;
+      pg += sg;
+      py += sy;
+    } else {
+      h0 = 0;
+      tok += step;
+      more = tok < a.tokens;
+      if (more) place();
+    }
+    on = more && h0 + hl < H && tok + (u32)tl < a.tokens;
+    xr.load(px, a.xs[z][3], e0, e1, has, a.D, on);
+    gr.load(pg, a.gs[z][3], e0, e1, has, a.D, on);
+
+    float ss = 0.0f, hx = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        load_raw<T, V>(rx[i], xp, a.xs[z][3], e0[i], e1[i], a.D, on && has[i]);
-        load_raw<T, V>(rg[i], gp, a.gs[z][3], e0[i], e1[i], a.D, on && has[i]);
+    for (int i = 0; i < NS; ++i) {
+      float c[V], sn[V], wa[V], wb[V];
+      const int p = has[i] ? p0 + 32 * i : 0;
+      read_row<V>(c_row, p, a.slots, c);
+      read_row<V>(c_row + row, p, a.slots, sn);
+      read_row<V>(w, p, a.slots, wa);
+      read_row<V>(w + row, p, a.slots, wb);
+      Lanes<V> A, B, C, S;
+      A.set(wa);
+      B.set(wb);
+      C.set(c);
+      S.set(sn);
+      Wide<V> s0 = Lanes<V>::all(0.0f), s1 = s0, q0 = s0, q1 = s0;
+#pragma unroll
+      for (int j = 0; j < Lanes<V>::N; ++j) {
+        const Wide<V> u = ga[i].x[j], v = gb[i].x[j];
+        ga[i].x[j] = fma(u, C.x[j], mul(v, mul(S.x[j], Lanes<V>::all(-1.0f))));
+        gb[i].x[j] = fma(v, C.x[j], mul(u, S.x[j]));
+        s0 = fma(xa[i].x[j], xa[i].x[j], s0);
+        s1 = fma(xb[i].x[j], xb[i].x[j], s1);
+        q0 = fma(mul(ga[i].x[j], xa[i].x[j]), A.x[j], q0);
+        q1 = fma(mul(gb[i].x[j], xb[i].x[j]), B.x[j], q1);
       }
-      float x0[NS][V], x1[NS][V], g0[NS][V], g1[NS][V];
-      float ss = 0.0f, hx = 0.0f;
+      ss += Lanes<V>::sum(s0) + Lanes<V>::sum(s1);
+      hx += Lanes<V>::sum(q0) + Lanes<V>::sum(q1);
+    }
+    ss = group_sum(ss, a.lanes);
+    hx = group_sum(hx, a.lanes);
+    const float r = now ? rsqrtf(fmaf(ss, inv_d, a.eps)) : 0.0f;
+    const Wide<V> rr = Lanes<V>::all(r), kk = Lanes<V>::all(-(r * r * r) * (hx * inv_d));
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        to_floats<T, V>(rx[i], x0[i], x1[i]);
-        to_floats<T, V>(rg[i], g0[i], g1[i]);
-        float c[V], s[V], w0[V], w1[V];
-        const int p = has[i] ? p0 + 32 * i : 0;
-        read_row<V>(cosine + t * row, p, a.slots, c);
-        read_row<V>(sine + t * row, p, a.slots, s);
-        rotate<V, ADJ>(g0[i], g1[i], c, s);
-        read_row<V>(w, p, a.slots, w0);
-        read_row<V>(w + row, p, a.slots, w1);
+    for (int i = 0; i < NS; ++i) {
+      float wa[V], wb[V], f[V], g[V];
+      const int p = has[i] ? p0 + 32 * i : 0;
+      read_row<V>(w, p, a.slots, wa);
+      read_row<V>(w + row, p, a.slots, wb);
+      Lanes<V> A, B;
+      A.set(wa);
+      B.set(wb);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          ss = fmaf(x0[i][j], x0[i][j], fmaf(x1[i][j], x1[i][j], ss));
-          hx = fmaf(g0[i][j] * w0[j], x0[i][j], fmaf(g1[i][j] * w1[j], x1[i][j], hx));
-        }
+      for (int j = 0; j < Lanes<V>::N; ++j) {
+        const Wide<V> g0 = mul(ga[i].x[j], rr), g1 = mul(gb[i].x[j], rr);
+        dwa[i].x[j] = fma(g0, xa[i].x[j], dwa[i].x[j]);
+        dwb[i].x[j] = fma(g1, xb[i].x[j], dwb[i].x[j]);
+        A.x[j] = fma(g0, A.x[j], mul(xa[i].x[j], kk));
+        B.x[j] = fma(g1, B.x[j], mul(xb[i].x[j], kk));
       }
-      for (int o = a.lanes >> 1; o; o >>= 1) {
-        ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        hx += __shfl_xor_sync(0xffffffffu, hx, o);
-      }
-      // a group without a row has r = rsqrt(eps) and zeros everywhere else: with eps = 0 that would be 0 * inf
-      const float r = on ? rsqrtf(ss / (float)a.D + a.eps) : 0.0f;
-      const float k = r * r * r * (hx / (float)a.D);
-      T* out = static_cast<T*>(a.y[z]) + offs[t][2] + h * a.ys[z][2];
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        float w0[V], w1[V];
-        const int p = has[i] ? p0 + 32 * i : 0;
-        read_row<V>(w, p, a.slots, w0);
-        read_row<V>(w + row, p, a.slots, w1);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          dw0[i][j] = fmaf(g0[i][j], x0[i][j] * r, dw0[i][j]);
-          dw1[i][j] = fmaf(g1[i][j], x1[i][j] * r, dw1[i][j]);
-          g0[i][j] = r * g0[i][j] * w0[j] - x0[i][j] * k;
-          g1[i][j] = r * g1[i][j] * w1[j] - x1[i][j] * k;
-        }
-        store_row<T, V>(out, a.ys[z][3], e0[i], e1[i], a.D, on && has[i], g0[i], g1[i]);
-      }
+      A.get(f);
+      B.get(g);
+      store_pairs<T, V, ADJ>(out, a.ys[z][3], e0[i], e1[i], a.D, now && has[i], f, g);
     }
   }
   if (!a.partial) return;
   // lanes with the same slots in a warp, then the warps
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* red = w + 2 * row;  // [warps][2 * row]
 #pragma unroll
-  for (int i = 0; i < NS; ++i)
+  for (int i = 0; i < NS; ++i) {
+    float f[V], g[V];
+    dwa[i].get(f);
+    dwb[i].get(g);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float s0 = dw0[i][j], s1 = dw1[i][j];
+      float s0 = f[j], s1 = g[j];
       for (int o = a.lanes; o < 32; o <<= 1) {
         s0 += __shfl_xor_sync(0xffffffffu, s0, o);
         s1 += __shfl_xor_sync(0xffffffffu, s1, o);
@@ -393,15 +592,16 @@ __global__ void __launch_bounds__(kRotThreads) rotary_grad_kernel(const __grid_c
         red[warp * 2 * row + row + (p0 + 32 * i) * V + j] = s1;
       }
     }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * row; i += kRotThreads) {
     float sum = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kRotThreads / 32; ++k) sum += red[k * 2 * row + i];
+    for (int k = 0; k < kRotWarps; ++k) sum += red[k * 2 * row + i];
     const int second = i >= row, f = i - second * row;
     int e[2];
-    slot_elems(a, f / V, V, &e[0], &e[1]);
-    const int el = e[second] + f % V;
+    pair_elems(a, f / V, f % V, V, &e[0], &e[1]);
+    const int el = e[second];
     if (el < a.D) a.partial[(i64)blockIdx.x * a.D + el] = sum;
   }
 }
@@ -506,22 +706,20 @@ static int slots_per_lane(const RotaryArgs& a) {
 template <class T, int V, int NS, bool ADJ>
 static int launch_forward(RotaryArgs& a, bool norm, cudaStream_t s) {
   set_slots(&a, V);
-  const int H = a.heads[0] + a.heads[1], groups = kRotThreads / a.lanes;
-  // rows per CTA: enough CTAs for every SM to hold several, at most eight rounds of the groups
+  const int H = a.heads[0] + a.heads[1], row = a.slots * V;
+  const int groups = 32 / a.lanes;
+  // rows per warp: what leaves 40 warps to an SM, between one round of the lane groups and kRotRounds
   const int64_t rows = (int64_t)a.tokens * H;
-  const int64_t want = std::min<int64_t>(std::max<int64_t>(rows / (sm_count() * 6), groups), 8 * groups);
-  if (H <= want) {
-    a.head_span = H;
-    a.tile = (int)std::min<int64_t>(std::max<int64_t>(want / H, 1), kRotMaxTile);
-  } else {
-    const int parts = (int)((H + want - 1) / want);
-    a.head_span = (H + parts - 1) / parts;
-    a.tile = 1;
-  }
-  const dim3 grid((a.tokens + a.tile - 1) / a.tile, (H + a.head_span - 1) / a.head_span);
-  const size_t smem = sizeof(float) * (size_t)a.slots * V * (2 * a.tile + (norm ? 4 : 0));
-  if (norm) rotary_kernel<T, V, NS, true, ADJ><<<grid, kRotThreads, smem, s>>>(a);
-  else rotary_kernel<T, V, NS, false, ADJ><<<grid, kRotThreads, smem, s>>>(a);
+  const int want = (int)std::min<int64_t>(std::max<int64_t>(rows / (sm_count() * 40), groups), kRotRounds * groups);
+  a.tile = std::max(1, std::min(std::min(want / H, kRotMaxTile), kRotTable / row));
+  a.parts = (H + want - 1) / want;
+  a.head_span = (H + a.parts - 1) / a.parts;
+  a.parts = (H + a.head_span - 1) / a.head_span;
+  const int64_t units = ((int64_t)a.tokens + a.tile - 1) / a.tile * a.parts, grid = (units + kRotWarps - 1) / kRotWarps;
+  TWG_REQUIRE(units + kRotWarps < (int64_t(1) << 32), "too many rows: %lld tokens of %d heads", (long long)a.tokens, H);
+  const size_t smem = sizeof(float) * (size_t)row * (2 * a.tile * kRotWarps + (norm ? 4 : 0));
+  if (norm) rotary_kernel<T, V, NS, true, ADJ><<<(unsigned)grid, kRotThreads, smem, s>>>(a);
+  else rotary_kernel<T, V, NS, false, ADJ><<<(unsigned)grid, kRotThreads, smem, s>>>(a);
   TWG_CHECK_LAUNCH();
   g_last_path = V == 1 ? kPathStrided64 : kPathDense;
   return TWG_OK;
@@ -570,36 +768,47 @@ static void grad_ctas(const TwgRotaryDesc* d, int* cq, int* ck) {
   *cq = *ck = 0;
   if (tokens == 0 || hq + hk == 0) return;
   const int64_t share = hq == 0 ? 0 : hk == 0 ? kRotGradCtas : std::min<int64_t>(std::max<int64_t>(kRotGradCtas * hq / (hq + hk), 1), kRotGradCtas - 1);
-  if (hq) *cq = (int)std::min<int64_t>(share, tokens);
-  if (hk) *ck = (int)std::min<int64_t>(kRotGradCtas - share, tokens);
+  const int64_t most = (tokens + kRotWarps - 1) / kRotWarps;  // a token to every warp
+  if (hq) *cq = (int)std::min<int64_t>(share, most);
+  if (hk) *ck = (int)std::min<int64_t>(kRotGradCtas - share, most);
+}
+
+// The workspace: the CTAs' partial sums, then (on a 256-byte boundary) the tables.
+static size_t grad_table_offset(const TwgRotaryDesc* d) {
+  int cq, ck;
+  grad_ctas(d, &cq, &ck);
+  return (std::max<size_t>(256, sizeof(float) * (size_t)(cq + ck) * (size_t)d->head_dim) + 255) / 256 * 256;
 }
 
 template <class T, int V, int NS, bool ADJ>
-static int launch_grad(RotaryArgs& a, cudaStream_t s) {
+static int launch_grad(RotaryArgs& a, float* table, cudaStream_t s) {
   set_slots(&a, V);
-  const int groups = kRotThreads / a.lanes;
-  // tokens per round: about four rounds of the groups, no more than an even share of the tokens
-  const int h = std::max(std::max(a.heads[0], a.heads[1]), 1), c = std::max(std::max(a.ctas[0], a.ctas[1]), 1);
-  a.tile = std::max(1, std::min(std::min(4 * groups / h, kRotMaxTile), (int)((a.tokens + c - 1) / c)));
-  // and tables, weights and the warps' sums within 47 KB of shared memory
-  constexpr int kFixedRows = 2 + 2 * (kRotThreads / 32);
-  a.tile = std::max(1, std::min(a.tile, (47 * 256 / (a.slots * V) - kFixedRows) / 2));
-  const size_t smem = sizeof(float) * (size_t)a.slots * V * (2 * a.tile + kFixedRows);
+  const int row = a.slots * V;
+  for (int t = 0; t < 2; ++t) {
+    a.step[t] = 1;
+    while (a.step[t] < a.heads[t] && a.step[t] < 32 / a.lanes) a.step[t] *= 2;
+  }
+  const int64_t grid = ((int64_t)a.tokens * row + kRotThreads - 1) / kRotThreads;
+  TWG_REQUIRE(grid <= 0x7fffffff, "too many tokens: %lld of %d frequencies", (long long)a.tokens, a.R / 2);
+  rotary_table_kernel<V><<<(unsigned)grid, kRotThreads, 0, s>>>(a, table);
+  TWG_CHECK_LAUNCH();
+  a.table = table;
+  const size_t smem = sizeof(float) * (size_t)row * (2 + 2 * kRotWarps);
   rotary_grad_kernel<T, V, NS, ADJ><<<a.ctas[0] + a.ctas[1], kRotThreads, smem, s>>>(a);
   TWG_CHECK_LAUNCH();
   g_last_path = V == 1 ? kPathStrided64 : kPathDense;
   return TWG_OK;
 }
 template <class T>
-static int backward(RotaryArgs& a, bool vec, cudaStream_t s) {
+static int backward(RotaryArgs& a, bool vec, float* table, cudaStream_t s) {
   constexpr int V = kVecOf<T>;
-  if (vec) return a.adjacent ? launch_grad<T, V, 1, true>(a, s) : launch_grad<T, V, 1, false>(a, s);
+  if (vec) return a.adjacent ? launch_grad<T, V, 1, true>(a, table, s) : launch_grad<T, V, 1, false>(a, table, s);
   set_slots(&a, 1);
   switch (slots_per_lane(a)) {
-    case 1: return launch_grad<T, 1, 1, false>(a, s);
-    case 2: return launch_grad<T, 1, 2, false>(a, s);
-    case 4: return launch_grad<T, 1, 4, false>(a, s);
-    default: return launch_grad<T, 1, 8, false>(a, s);
+    case 1: return launch_grad<T, 1, 1, false>(a, table, s);
+    case 2: return launch_grad<T, 1, 2, false>(a, table, s);
+    case 4: return launch_grad<T, 1, 4, false>(a, table, s);
+    default: return launch_grad<T, 1, 8, false>(a, table, s);
   }
 }
 
@@ -622,9 +831,7 @@ extern "C" int twg_qk_norm_rotary(const TwgRotaryDesc* d, const void* q, const v
 
 extern "C" size_t twg_qk_norm_rotary_workspace_bytes(const TwgRotaryDesc* d) {
   if (check_rotary("twg_qk_norm_rotary_workspace_bytes", d) != TWG_OK) return 0;
-  int cq, ck;
-  grad_ctas(d, &cq, &ck);
-  return std::max<size_t>(256, sizeof(float) * (size_t)(cq + ck) * (size_t)d->head_dim);
+  return grad_table_offset(d) + sizeof(float) * 2 * (size_t)(d->batch * d->seq) * (size_t)((d->head_dim + 1) / 2);
 }
 
 extern "C" int twg_qk_norm_rotary_backward(const TwgRotaryDesc* d, const void* q, const void* k, const void* q_weight,
@@ -650,12 +857,11 @@ extern "C" int twg_qk_norm_rotary_backward(const TwgRotaryDesc* d, const void* q
     const size_t e = (size_t)float_size(d->dtype);
     TWG_REQUIRE(is_aligned(q, e) && is_aligned(k, e) && is_aligned(dq_out, e) && is_aligned(dk_out, e) && is_aligned(dq, e) && is_aligned(dk, e),
                 "%s: a tensor is not aligned to its elements", name);
-    if (sums) {
-      const size_t need = twg_qk_norm_rotary_workspace_bytes(d);
-      TWG_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes is smaller than the %zu needed", name,
-                  workspace ? workspace_bytes : (size_t)0, need);
-      TWG_REQUIRE(is_aligned(workspace, 16), "%s: workspace must be 16-byte aligned", name);
-    }
+    const size_t need = twg_qk_norm_rotary_workspace_bytes(d);
+    TWG_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes is smaller than the %zu needed", name,
+                workspace ? workspace_bytes : (size_t)0, need);
+    TWG_REQUIRE(is_aligned(workspace, 16), "%s: workspace must be 16-byte aligned", name);
+    float* table = reinterpret_cast<float*>(static_cast<char*>(workspace) + grad_table_offset(d));
     a.x[0] = q; a.x[1] = k; a.g[0] = dq_out; a.g[1] = dk_out; a.y[0] = dq; a.y[1] = dk;
     a.w[0] = q_weight; a.w[1] = k_weight;
     a.pos = positions;
@@ -663,7 +869,7 @@ extern "C" int twg_qk_norm_rotary_backward(const TwgRotaryDesc* d, const void* q
     a.sign = -1.0f;
     a.partial = sums ? static_cast<float*>(workspace) : nullptr;
     vec = vec && rows_aligned(a, true);
-    const int rc = dispatch_float(d->dtype, [&](auto* t) { return backward<std::remove_pointer_t<decltype(t)>>(a, vec, s); });
+    const int rc = dispatch_float(d->dtype, [&](auto* t) { return backward<std::remove_pointer_t<decltype(t)>>(a, vec, table, s); });
     if (rc != TWG_OK) return rc;
   }
   if (!sums) return TWG_OK;

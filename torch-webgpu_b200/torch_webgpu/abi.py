@@ -11,6 +11,7 @@ the result; they exist so that parity tests and small scripts can drive the C AB
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import POINTER, byref, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 
@@ -353,6 +354,10 @@ def make_desc(shape, operands) -> IterDesc:
     return d
 
 
+_ROTARY_LAYOUT = struct.Struct(f"9if31q{ROTARY_MAX_FREQS}s")  # RotaryDesc, field by field
+_NO_STRIDES = ((0, 0, 0, 0), (0, 0, 0, 0))
+
+
 def rotary_desc(dtype: str, tokens, heads, head_dim: int, *, in_strides, out_strides, position_strides, grad_strides=None,
                 rot_dim: int | None = None, axes: int = 1, axis_of=None, adjacent: bool = False, inverse: bool = False,
                 eps: float = 1e-6, weight_dtype: str = "float32", position_dtype: str = "int64",
@@ -364,22 +369,14 @@ def rotary_desc(dtype: str, tokens, heads, head_dim: int, *, in_strides, out_str
     names each frequency's axis (default: axis 0).  Types are names of DTYPES.
     """
     rot_dim = head_dim if rot_dim is None else rot_dim
-    d = RotaryDesc(DTYPES[dtype], DTYPES[weight_dtype], DTYPES[position_dtype], DTYPES[freq_dtype], head_dim, rot_dim, axes,
-                   int(adjacent), int(inverse), eps, tokens[0], tokens[1])
-    d.heads[:] = heads
-    for t in range(2):
-        d.in_strides[t][:] = in_strides[t]
-        d.out_strides[t][:] = out_strides[t]
-        if grad_strides is not None:
-            d.grad_strides[t][:] = grad_strides[t]
-    d.position_strides[:] = position_strides
-    if axis_of is not None:
-        if len(axis_of) != rot_dim // 2 or len(axis_of) > ROTARY_MAX_FREQS:
-            raise TwgError(TWG_ERR_INVALID, f"axis_of names {len(axis_of)} axes for {rot_dim // 2} frequencies")
-        if len(axis_of) and not 0 <= min(axis_of) <= max(axis_of) < axes:
-            raise TwgError(TWG_ERR_INVALID, f"axis_of must name axes 0..{axes - 1}")
-        ctypes.memmove(d.axis_of, bytes(axis_of), len(axis_of))
-    return d
+    table = b"" if axis_of is None else bytes(axis_of)
+    if axis_of is not None and (len(table) != rot_dim // 2 or len(table) > ROTARY_MAX_FREQS or table.strip(bytes(range(axes)))):
+        raise TwgError(TWG_ERR_INVALID, f"axis_of must name one of the {axes} axes for each of the {rot_dim // 2} frequencies")
+    grads = _NO_STRIDES if grad_strides is None else grad_strides
+    # packed at once: a field at a time costs several microseconds of a call
+    return RotaryDesc.from_buffer_copy(_ROTARY_LAYOUT.pack(
+        DTYPES[dtype], DTYPES[weight_dtype], DTYPES[position_dtype], DTYPES[freq_dtype], head_dim, rot_dim, axes, adjacent, inverse, eps,
+        *tokens, *heads, *in_strides[0], *in_strides[1], *out_strides[0], *out_strides[1], *grads[0], *grads[1], *position_strides, table))
 
 
 def logprobs_desc(dtype: str, rows: int, vocab: int, *, row_stride: int | None = None, tokens_per_row: int = 1, token_strides=None,

@@ -39,6 +39,55 @@ __device__ __forceinline__ void philox_block(u64 block, u64 seed, u64 offset, u3
   r[0] = c0; r[1] = c1; r[2] = c2; r[3] = c3;
 }
 
+// What does not depend on the block's number, for blocks below 2^32: the keys of ten rounds and the
+// products of the first two, folded into one word for each exclusive or.  In the kernel's arguments
+// they cost no instruction; worked out by every thread they were 4 of 23 instructions an element.
+struct PhiloxPlan {
+  u32 x[10][2];  // what words 0 and 2 of each round are combined with besides the products' halves
+};
+static PhiloxPlan make_plan(u64 seed, u64 offset) {
+  PhiloxPlan p;
+  u32 k0 = (u32)seed, k1 = (u32)(seed >> 32);
+  for (int i = 0; i < 10; ++i) {
+    p.x[i][0] = k0;
+    p.x[i][1] = k1;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  const u64 b = (u64)(u32)offset * 0xCD9E8D57u;      // round 0: word 2 is the offset's low word, word 1 is zero
+  const u32 w0 = (u32)(b >> 32) ^ p.x[0][0], w1 = (u32)b;
+  p.x[0][1] ^= (u32)(offset >> 32);
+  const u64 a = (u64)w0 * 0xD2511F53u;               // round 1: word 0 is w0
+  p.x[1][0] ^= w1;
+  p.x[1][1] ^= (u32)(a >> 32);
+  p.x[2][1] ^= (u32)a;                               // round 2: word 3
+  return p;
+}
+__device__ __forceinline__ void philox_planned(u32 block, const PhiloxPlan& p, u32 (&r)[4]) {
+  u64 a = (u64)block * 0xD2511F53u, b;
+  u32 c0, c1, c2 = (u32)(a >> 32) ^ p.x[0][1], c3 = (u32)a;  // round 0
+  b = (u64)c2 * 0xCD9E8D57u;
+  c0 = (u32)(b >> 32) ^ p.x[1][0];                           // round 1
+  c1 = (u32)b;
+  c2 = c3 ^ p.x[1][1];
+  a = (u64)c0 * 0xD2511F53u;
+  b = (u64)c2 * 0xCD9E8D57u;
+  c0 = (u32)(b >> 32) ^ c1 ^ p.x[2][0];                      // round 2
+  c1 = (u32)b;
+  c2 = (u32)(a >> 32) ^ p.x[2][1];
+  c3 = (u32)a;
+#pragma unroll
+  for (int i = 3; i < 10; ++i) {
+    a = (u64)c0 * 0xD2511F53u;
+    b = (u64)c2 * 0xCD9E8D57u;
+    c0 = (u32)(b >> 32) ^ c1 ^ p.x[i][0];
+    c2 = (u32)(a >> 32) ^ c3 ^ p.x[i][1];
+    c1 = (u32)b;
+    c3 = (u32)a;
+  }
+  r[0] = c0; r[1] = c1; r[2] = c2; r[3] = c3;
+}
+
 __device__ __forceinline__ void load_state(const DropoutArgs& a, u64* seed, u64* offset) {
   *seed = a.state ? a.state[0] : a.seed;
   *offset = a.state ? a.state[1] + a.offset : a.offset;
@@ -48,14 +97,14 @@ __device__ __forceinline__ float drop(const DropoutArgs& a, u32 word, float x) {
   return word >= a.threshold && !a.drop_all ? x * a.scale : 0.0f;
 }
 
-constexpr int kDropUnroll = 2;  // 16-byte vectors per thread
+constexpr int kDropUnroll = 4;  // 16-byte vectors per thread
 
-// Dense operands: `vecs` whole 16-byte vectors; the last CTA also takes the tail of n.
+// Dense operands of fewer than 2^34 elements, the seed and offset from the host and p below 1: `vecs`
+// whole 16-byte vectors; the last CTA also takes the tail of n.
 template <class T, bool RES>
-__global__ void __launch_bounds__(kBlock) dropout_dense_kernel(const __grid_constant__ DropoutArgs a, i64 vecs, i64 n) {
+__global__ void __launch_bounds__(kBlock) dropout_dense_kernel(const __grid_constant__ DropoutArgs a, const __grid_constant__ PhiloxPlan plan,
+                                                                i64 vecs, i64 n) {
   constexpr int V = kVecOf<T>;
-  u64 seed, offset;
-  load_state(a, &seed, &offset);
   const T* x = static_cast<const T*>(a.x);
   const T* res = static_cast<const T*>(a.residual);
   T* out = static_cast<T*>(a.out);
@@ -79,10 +128,10 @@ __global__ void __launch_bounds__(kBlock) dropout_dense_kernel(const __grid_cons
 #pragma unroll
     for (int b = 0; b < V / 4; ++b) {
       u32 w[4];
-      philox_block((u64)v * (V / 4) + b, seed, offset, w);
+      philox_planned((u32)v * (u32)(V / 4) + (u32)b, plan, w);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float d = drop(a, w[j], f[4 * b + j]);
+        const float d = w[j] >= a.threshold ? f[4 * b + j] * a.scale : 0.0f;
         if constexpr (RES) y[4 * b + j] += d;
         else y[4 * b + j] = d;
       }
@@ -93,14 +142,16 @@ __global__ void __launch_bounds__(kBlock) dropout_dense_kernel(const __grid_cons
   if (blockIdx.x == gridDim.x - 1 && tail + threadIdx.x < n) {
     const i64 i = tail + threadIdx.x;
     u32 w[4];
-    philox_block((u64)i >> 2, seed, offset, w);
-    float y = drop(a, i & 2 ? (i & 1 ? w[3] : w[2]) : (i & 1 ? w[1] : w[0]), to_f32(x[i]));
+    philox_planned((u32)(i >> 2), plan, w);
+    const u32 word = i & 2 ? (i & 1 ? w[3] : w[2]) : (i & 1 ? w[1] : w[0]);
+    float y = word >= a.threshold ? to_f32(x[i]) * a.scale : 0.0f;
     if constexpr (RES) y += to_f32(res[i]);
     out[i] = from_f32<T>(y);
   }
 }
 
-// Any strides: a thread takes the four elements of one block, one after the other along dimension 0.
+// Any strides, a seed on the device, p = 1: a thread takes the four elements of one block, one after the
+// other along dimension 0.
 template <class T, bool RES, class IDX>
 __global__ void __launch_bounds__(kBlock) dropout_strided_kernel(const __grid_constant__ DropoutArgs a, const __grid_constant__ StridedDesc<3, IDX> d, i64 n) {
   u64 seed, offset;
@@ -137,8 +188,8 @@ static int launch_dropout(const DropoutArgs& a, const TwgIterDesc& d, cudaStream
   if (dense) {
     const i64 vecs = d.numel / V, per = kBlock * kDropUnroll;
     const i64 grid = std::max<i64>(1, (vecs + per - 1) / per);
-    if (grid <= 0x7fffffff) {
-      dropout_dense_kernel<T, RES><<<(unsigned)grid, kBlock, 0, s>>>(a, vecs, d.numel);
+    if (d.numel < (i64(1) << 34) && !a.state && !a.drop_all) {
+      dropout_dense_kernel<T, RES><<<(unsigned)grid, kBlock, 0, s>>>(a, make_plan(a.seed, a.offset), vecs, d.numel);
       TWG_CHECK_LAUNCH();
       g_last_path = kPathDense;
       return TWG_OK;

@@ -25,9 +25,11 @@ namespace twg {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLpMaxThreads = 512;
+constexpr int kLpMaxThreads = 256;
 constexpr int kLpMaxWarps = kLpMaxThreads / 32;
 constexpr int kLpUnroll = 4;       // 16-byte vectors a thread has in flight
+constexpr int kLpGradUnroll = 8;   // the same of the gradient
+constexpr int kLpGradRounds = 2;   // rounds of its loads in a CTA
 constexpr int kLpMaxCluster = 8;
 constexpr int kLpMaxTop = 32;
 constexpr int kLpCandidates = 1024;
@@ -83,6 +85,37 @@ struct Soft {
       s += __shfl_xor_sync(0xffffffffu, s, o);
       t += __shfl_xor_sync(0xffffffffu, t, o);
     }
+  }
+};
+
+// The same while a thread collects them, in two halves that one instruction works on.
+struct SoftPair {
+  float m;
+  Two s, t;
+  __device__ __forceinline__ SoftPair() : m(-FLT_MAX), s(0.0f, 0.0f), t(0.0f, 0.0f) {}
+  template <int N>
+  __device__ __forceinline__ void add_all(const float (&f)[N], float largest, float c) {
+    const float to = fmaxf(m, largest), d = hold((m - to) * c), r = ex2(d);
+    const Two rr(r, r), cc(c, c), base(-to, -to);
+    t = mul(rr, fma(Two(d, d), s, t));
+    s = mul(rr, s);
+    m = to;
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      float u0, u1;
+      mul(add(Two(f[j], f[j + 1]), base), cc).get(u0, u1);
+      u0 = hold(u0);
+      u1 = hold(u1);
+      const Two e(ex2(u0), ex2(u1));
+      s = add(s, e);
+      t = fma(e, Two(u0, u1), t);
+    }
+  }
+  __device__ __forceinline__ Soft sum() const {
+    float s0, s1, t0, t1;
+    s.get(s0, s1);
+    t.get(t0, t1);
+    return Soft{m, s0 + s1, t0 + t1};
   }
 };
 
@@ -197,7 +230,7 @@ __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const __grid_co
   const int i_extra = tid < rs.head ? tid : a.vocab - rs.tail + tid - rs.head;
   float fx[1] = {extra ? to_f32(row[i_extra]) : -INFINITY};
 
-  Soft soft = no_soft();
+  SoftPair mine;
   float limit = INFINITY;  // only elements that reach it can be among the alternatives
   auto push = [&](float x, int index) {
     if (x >= limit) {
@@ -205,26 +238,32 @@ __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const __grid_co
       if (at < kLpCandidates) sh.found[at] = rank_key(x, (u32)index);
     }
   };
-  bool first = true;
-  for (int base = v0; base < v1 || first; base += nt * kLpUnroll) {
-    uint4 raw[kLpUnroll];
+  uint4 raw[kLpUnroll];
+  auto fetch = [&](int base) {
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k) {
       const int v = base + k * nt + tid;
-      raw[k] = v < v1 ? ld_v4(row + rs.head + (i64)v * V) : minus_inf<T>();
+      raw[k] = minus_inf<T>();
+      if (v < v1) raw[k] = ld_v4(row + rs.head + (i64)v * V);
     }
-    float largest = -INFINITY, f[kLpUnroll][V];
+  };
+  fetch(v0);
+  bool first = true;
+  for (int base = v0; base < v1 || first; base += nt * kLpUnroll) {
+    float largest = -INFINITY, f[kLpUnroll * V];
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k) {
-      unpack(raw[k], f[k], static_cast<const T*>(nullptr));
+      float g[V];
+      unpack(raw[k], g, static_cast<const T*>(nullptr));
 #pragma unroll
-      for (int j = 0; j < V; ++j) largest = fmaxf(largest, f[k][j]);
+      for (int j = 0; j < V; ++j) {
+        f[k * V + j] = g[j];
+        largest = fmaxf(largest, g[j]);
+      }
     }
-    soft.rebase(fmaxf(soft.m, largest), c);
-#pragma unroll
-    for (int k = 0; k < kLpUnroll; ++k) soft.add(f[k], soft.m, c);
+    if (base + nt * kLpUnroll < v1) fetch(base + nt * kLpUnroll);  // on its way while this round is summed
+    mine.add_all(f, largest, c);
     if (first) {
-      soft.add(fx, fx[0], c);
       if constexpr (TOP) {
         // A bound below which no element can be among the `top` largest: that many threads have seen
         // one above it.  The largest 16-bit prefix of the threads' maxima that `top` of them reach.
@@ -250,12 +289,14 @@ __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const __grid_co
           const int v = base + k * nt + tid;
           if (v < v1) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) push(f[k][j], rs.head + v * V + j);
+            for (int j = 0; j < V; ++j) push(f[k * V + j], rs.head + v * V + j);
           }
         }
       }
     }
   }
+  Soft soft = mine.sum();
+  soft.add(fx, fx[0], c);
 
   if constexpr (TOP) {
     const bool nan = __syncthreads_or(soft.s != soft.s) != 0;
@@ -379,9 +420,9 @@ __global__ void __launch_bounds__(256) logprobs_grad_kernel(const __grid_constan
     const i64 at = r * a.ts0 + j * a.ts1;
     return a.tok64 ? static_cast<const i64*>(a.tokens)[at] : (i64) static_cast<const int*>(a.tokens)[at];
   };
-  uint4 raw[kLpUnroll];
+  uint4 raw[kLpGradUnroll];
 #pragma unroll
-  for (int k = 0; k < kLpUnroll; ++k) {
+  for (int k = 0; k < kLpGradUnroll; ++k) {
     const int v = v0 + k * nt + tid;
     if (v < v1) raw[k] = ld_v4(row + rs.head + (i64)v * V);
   }
@@ -401,43 +442,57 @@ __global__ void __launch_bounds__(256) logprobs_grad_kernel(const __grid_constan
   const float A = (a.dlse ? a.dlse[r] : 0.0f) - g;
   const float c = a.scale * kLog2e;
   float m = 0.0f, off = lse * kLog2e;
-  bool none = false;  // no finite logit: no distribution, no gradient
   if (fabsf(lse) > kLpFarLse) {
     const Soft soft = row_softmax<T>(row, rs, a.vocab, c);
     m = soft.m;
-    off = log2f(soft.s);
-    none = soft.s == 0.0f;
+    // no finite logit: no distribution, no gradient; every p becomes 0
+    off = soft.s == 0.0f ? INFINITY : log2f(soft.s);
   }
   // with u = ln p / ln 2: dx = 2^u (slope u + level)
   const float slope = -dH * kLn2 * a.scale, level = (A - dH * H) * a.scale;
-  auto grad = [&](float x) {
-    const float u = hold(fmaf(x - m, c, -off));
-    return none ? 0.0f : ex2(u) * fmaf(slope, u, level);
+  const Two minus_m(-m, -m), cc(c, c), minus_off(-off, -off), slopes(slope, slope), levels(level, level);
+  auto grad = [&](float& x0, float& x1) {
+    float u0, u1;
+    fma(add(Two(x0, x1), minus_m), cc, minus_off).get(u0, u1);
+    u0 = hold(u0);
+    u1 = hold(u1);
+    mul(Two(ex2(u0), ex2(u1)), fma(slopes, Two(u0, u1), levels)).get(x0, x1);
   };
   const bool wide = ((reinterpret_cast<u64>(row) ^ reinterpret_cast<u64>(out)) & 15u) == 0;
-  for (int base = v0; base < v1; base += nt * kLpUnroll) {
+  for (int base = v0; base < v1; base += nt * kLpGradUnroll) {
+    float f[kLpGradUnroll][V];
 #pragma unroll
-    for (int k = 0; k < kLpUnroll; ++k) {
+    for (int k = 0; k < kLpGradUnroll; ++k) {
+      if (base != v0) {
+        const int v = base + k * nt + tid;
+        if (v < v1) raw[k] = ld_v4(row + rs.head + (i64)v * V);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kLpGradUnroll; ++k) {
       const int v = base + k * nt + tid;
       if (v >= v1) break;
-      if (base != v0) raw[k] = ld_v4(row + rs.head + (i64)v * V);
-      float f[V];
-      unpack(raw[k], f, static_cast<const T*>(nullptr));
+      unpack(raw[k], f[k], static_cast<const T*>(nullptr));
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[j] = grad(f[j]);
+      for (int j = 0; j < V; j += 2) grad(f[k][j], f[k][j + 1]);
       T* to = out + rs.head + (i64)v * V;
-      if (wide) st_v4(to, pack(f, static_cast<const T*>(nullptr)));
+      if (wide) st_v4(to, pack(f[k], static_cast<const T*>(nullptr)));
       else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) to[j] = from_f32<T>(f[j]);
+        for (int j = 0; j < V; ++j) to[j] = from_f32<T>(f[k][j]);
       }
     }
   }
+  auto grad_at = [&](i64 i) {
+    float x = to_f32(row[i]), y = x;
+    grad(x, y);
+    return x;
+  };
   if (part == 0 && tid < rs.head + rs.tail) {
     const int i = tid < rs.head ? tid : a.vocab - rs.tail + tid - rs.head;
-    out[i] = from_f32<T>(grad(to_f32(row[i])));
+    out[i] = from_f32<T>(grad_at(i));
   }
-  if (!a.dlogp || none) return;
+  if (!a.dlogp || off == INFINITY) return;
   // The tokens' own elements again, with their share: computed in full and rounded once.  The CTA
   // that wrote the element writes it again, and of equal tokens the first one stands for all.
   __syncthreads();
@@ -454,7 +509,7 @@ __global__ void __launch_bounds__(256) logprobs_grad_kernel(const __grid_constan
       if (i < j) mine = false;
       sum += a.dlogp[r * a.m + i];
     }
-    if (mine) out[tok] = from_f32<T>(fmaf(sum, a.scale, grad(to_f32(row[tok]))));
+    if (mine) out[tok] = from_f32<T>(fmaf(sum, a.scale, grad_at(tok)));
   }
 }
 
@@ -502,9 +557,13 @@ template <class T>
 static int launch_logprobs_grad(LogprobGradArgs& a, int64_t rows, cudaStream_t s) {
   const int nvec = std::max(1, a.vocab / kVecOf<T>);
   int threads = 64;
-  while (threads < 256 && threads * kLpUnroll < nvec) threads *= 2;
+  while (threads < 256 && threads * kLpGradUnroll < nvec) threads *= 2;
   // one round of loads per CTA, two where that would be too many CTAs for the grid
-  int64_t parts = (nvec + threads * kLpUnroll - 1) / (threads * kLpUnroll);
+  // one round of loads in a CTA, or kLpGradRounds where the rows still make eight CTAs for every SM: what a
+  // CTA does before its first element counts for less then
+  const int64_t rounds = rows * nvec >= (int64_t)sm_count() * 8 * threads * kLpGradUnroll * kLpGradRounds ? kLpGradRounds : 1;
+  const int64_t each = threads * kLpGradUnroll * rounds;
+  int64_t parts = (nvec + each - 1) / each;
   while (parts > 1 && rows * parts > 0x7fffffff) parts = (parts + 1) / 2;
   a.parts = (int)parts;
   logprobs_grad_kernel<T><<<(unsigned)(rows * parts), threads, 0, s>>>(a);

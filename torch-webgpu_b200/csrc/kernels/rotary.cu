@@ -186,26 +186,9 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
   return v;
 }
 
-// Arithmetic on neighbours j, j + 1 of a lane's arrays in one instruction, where both are in
-// registers side by side (V > 1).  The kernels issue three instructions for two of the copy's rate
-// in scalar form; V == 1 keeps that form.
-struct Two {
-  u64 v;
-  __device__ __forceinline__ Two() {}
-  __device__ __forceinline__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
-  __device__ __forceinline__ void get(float& x, float& y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-};
-__device__ __forceinline__ Two mul(Two a, Two b) {
-  Two r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
-  Two r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-// A lane's V values as they are computed with: pairs of them, or the one.
+// A lane's V values as they are computed with: two in an instruction, where neighbours are in registers
+// side by side, or the one of the element path.  (In scalar form the kernels issued three instructions
+// for every two of this one.)
 template <int V>
 struct Lanes {
   static constexpr int N = V / 2;

@@ -66,6 +66,29 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8], const __nv_bfloat16*)
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Two float32 values in one register pair, and arithmetic on both in one instruction.
+struct Two {
+  u64 v;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ void get(float& x, float& y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+};
+__device__ __forceinline__ Two add(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 // Host side: bytes of a floating element type this family of kernels takes, 0 for any other.
 inline int float_size(int dtype) {
   return dtype == TWG_DTYPE_F32 ? 4 : (dtype == TWG_DTYPE_F16 || dtype == TWG_DTYPE_BF16) ? 2 : 0;

@@ -27,8 +27,10 @@ namespace cg = cooperative_groups;
 
 constexpr int kLpMaxThreads = 256;
 constexpr int kLpMaxWarps = kLpMaxThreads / 32;
-constexpr int kLpUnroll = 4;       // 16-byte vectors a thread has in flight
-constexpr int kLpGradUnroll = 8;   // the same of the gradient
+constexpr int kLpUnroll = 2;       // 16-byte vectors of a thread in one stage of the forward kernel's loads
+constexpr int kLpStages = 4;       // stages on their way (a power of two)
+constexpr int kLpCtas = 5;         // CTAs of that size an SM holds
+constexpr int kLpGradUnroll = 8;   // vectors a thread of the gradient has on their way
 constexpr int kLpGradRounds = 2;   // rounds of its loads in a CTA
 constexpr int kLpMaxCluster = 8;
 constexpr int kLpMaxTop = 32;
@@ -161,6 +163,10 @@ __device__ __forceinline__ uint4 minus_inf() {
   return make_uint4(w, w, w, w);
 }
 
+__device__ __forceinline__ void copy_async(uint4* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((u32)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+
 // Alternatives the slow way, for rows whose quick bound lets too many elements through (long runs
 // of equal logits, rising logits) or that hold a NaN: every warp keeps a sorted list in its lanes.
 template <class T>
@@ -208,9 +214,10 @@ __device__ __forceinline__ void rank_keys(const u64* keys, int n, int top, u64* 
 }
 
 template <class T, bool TOP>
-__global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+__global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
   constexpr int V = kVecOf<T>;
   __shared__ LpShared sh;
+  extern __shared__ uint4 ring[];  // [kLpStages][kLpUnroll][threads]
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const i64 r = blockIdx.x / (unsigned)parts;
@@ -238,55 +245,66 @@ __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const __grid_co
       if (at < kLpCandidates) sh.found[at] = rank_key(x, (u32)index);
     }
   };
-  uint4 raw[kLpUnroll];
-  auto fetch = [&](int base) {
+  // Every thread copies its own vectors to its own places in shared memory and reads them back, so a
+  // stage needs no barrier, and what is on its way takes no registers.
+  const int each = nt * kLpUnroll, n = v1 - v0;
+  auto fetch = [&](int q) {
+    uint4* to = ring + (q & (kLpStages - 1)) * each + tid;
+    const int v = v0 + q * each + tid;
 #pragma unroll
-    for (int k = 0; k < kLpUnroll; ++k) {
-      const int v = base + k * nt + tid;
-      raw[k] = minus_inf<T>();
-      if (v < v1) raw[k] = ld_v4(row + rs.head + (i64)v * V);
-    }
+    for (int k = 0; k < kLpUnroll; ++k)
+      if (v + k * nt < v1) copy_async(to + k * nt, row + rs.head + (i64)(v + k * nt) * V);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  fetch(v0);
-  bool first = true;
-  for (int base = v0; base < v1 || first; base += nt * kLpUnroll) {
-    float largest = -INFINITY, f[kLpUnroll * V];
+  auto take = [&](int q, float (&f)[kLpUnroll * V]) {
+    const uint4* from = ring + (q & (kLpStages - 1)) * each + tid;
+    const int v = v0 + q * each + tid;
+    float largest = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k) {
+      uint4 raw = minus_inf<T>();
+      if (v + k * nt < v1) raw = from[k * nt];
       float g[V];
-      unpack(raw[k], g, static_cast<const T*>(nullptr));
+      unpack(raw, g, static_cast<const T*>(nullptr));
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         f[k * V + j] = g[j];
         largest = fmaxf(largest, g[j]);
       }
     }
-    if (base + nt * kLpUnroll < v1) fetch(base + nt * kLpUnroll);  // on its way while this round is summed
-    mine.add_all(f, largest, c);
-    if (first) {
-      if constexpr (TOP) {
-        // A bound below which no element can be among the `top` largest: that many threads have seen
-        // one above it.  The largest 16-bit prefix of the threads' maxima that `top` of them reach.
-        const bool some = base + tid < v1;
-        u32 own = 0;
-        if (some) own = order_of(largest) >> 16;
-        if (extra) own = max(own, order_of(fx[0]) >> 16);
-        if (own > 0xff80u) own = 0xff80u;  // a NaN: the slow way will see it
-        u32 prefix = 0;
-        for (int bit = 15; bit >= 0; --bit) {
-          const u32 probe = prefix | (1u << bit);
-          if (__syncthreads_count(own >= probe) >= a.top) prefix = probe;
-        }
-        limit = prefix <= 0x7fu ? -INFINITY : value_of(prefix << 16);
-        if (extra) push(fx[0], i_extra);
-      }
-      first = false;
+    return largest;
+  };
+#pragma unroll
+  for (int q = 0; q < kLpStages; ++q) fetch(q);
+  float f[kLpUnroll * V];
+  if constexpr (TOP) {
+    // A bound below which no element can be among the `top` largest: that many threads have one above
+    // it in the first stages.  The largest 16-bit prefix of the threads' maxima that `top` of them reach.
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    float largest = fx[0];
+#pragma unroll 1
+    for (int q = 0; q < kLpStages; ++q) largest = fmaxf(largest, take(q, f));
+    u32 own = extra || tid < n ? order_of(largest) >> 16 : 0;
+    if (own > 0xff80u) own = 0xff80u;  // a NaN: the slow way will see it
+    u32 prefix = 0;
+    for (int bit = 15; bit >= 0; --bit) {
+      const u32 probe = prefix | (1u << bit);
+      if (__syncthreads_count(own >= probe) >= a.top) prefix = probe;
     }
+    limit = prefix <= 0x7fu ? -INFINITY : value_of(prefix << 16);
+    if (extra) push(fx[0], i_extra);
+  }
+#pragma unroll 1
+  for (int q = 0; q * each < n; ++q) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kLpStages - 1) : "memory");
+    const float largest = take(q, f);
+    fetch(q + kLpStages);
+    mine.add_all(f, largest, c);
     if constexpr (TOP) {
       if (largest >= limit) {
 #pragma unroll
         for (int k = 0; k < kLpUnroll; ++k) {
-          const int v = base + k * nt + tid;
+          const int v = v0 + q * each + k * nt + tid;
           if (v < v1) {
 #pragma unroll
             for (int j = 0; j < V; ++j) push(f[k * V + j], rs.head + v * V + j);
@@ -295,6 +313,7 @@ __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const __grid_co
       }
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   Soft soft = mine.sum();
   soft.add(fx, fx[0], c);
 
@@ -542,6 +561,7 @@ static int launch_logprobs(const LogprobArgs& a, int64_t rows, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * parts));
   cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = sizeof(uint4) * kLpStages * kLpUnroll * (size_t)threads;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -163,10 +163,6 @@ __device__ __forceinline__ uint4 minus_inf() {
   return make_uint4(w, w, w, w);
 }
 
-__device__ __forceinline__ void copy_async(uint4* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((u32)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-
 // Alternatives the slow way, for rows whose quick bound lets too many elements through (long runs
 // of equal logits, rising logits) or that hold a NaN: every warp keeps a sorted list in its lanes.
 template <class T>
@@ -254,7 +250,7 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k)
       if (v + k * nt < v1) copy_async(to + k * nt, row + rs.head + (i64)(v + k * nt) * V);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    copy_async_commit();
   };
   auto take = [&](int q, float (&f)[kLpUnroll * V]) {
     const uint4* from = ring + (q & (kLpStages - 1)) * each + tid;
@@ -280,7 +276,7 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
   if constexpr (TOP) {
     // A bound below which no element can be among the `top` largest: that many threads have one above
     // it in the first stages.  The largest 16-bit prefix of the threads' maxima that `top` of them reach.
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    copy_async_wait<0>();
     float largest = fx[0];
 #pragma unroll 1
     for (int q = 0; q < kLpStages; ++q) largest = fmaxf(largest, take(q, f));
@@ -296,7 +292,7 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
   }
 #pragma unroll 1
   for (int q = 0; q * each < n; ++q) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kLpStages - 1) : "memory");
+    copy_async_wait<kLpStages - 1>();
     const float largest = take(q, f);
     fetch(q + kLpStages);
     mine.add_all(f, largest, c);
@@ -313,7 +309,7 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
       }
     }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  copy_async_wait<0>();
   Soft soft = mine.sum();
   soft.add(fx, fx[0], c);
 

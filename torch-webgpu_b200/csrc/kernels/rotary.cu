@@ -21,6 +21,7 @@ constexpr int kRotWarps = kRotThreads / 32;
 constexpr int kRotRounds = 10;         // rows of a lane group in a warp's tile, where there are enough
 constexpr int kRotMaxTile = 16;        // tokens in such a tile
 constexpr int kRotTable = 512;         // entries of its tables
+constexpr int kRotStages = 2;          // rounds of the gradient's rows on their way
 constexpr int kRotMaxDim = 512;
 constexpr int kRotMaxAxes = 8;
 constexpr int kRotGradCtas = 148 * 2;  // CTAs of the gradient kernel: one row of weight partial sums each
@@ -79,17 +80,39 @@ __device__ __forceinline__ void token_place(const RotaryArgs& a, u32 tok, i64* b
   *s = tok - q * a.seq;
 }
 
+// Sine and cosine of an angle in 2^-32 turns.  The two top bits round to a quarter turn; what is left
+// is at most pi / 4, where the Taylor series reach float32 with y^9 and y^10 (the next terms are below
+// 2^-28 of the result), and the quarters swap and negate them.
+__device__ __forceinline__ void turn_sincos(u32 turn, float* s, float* c) {
+  const u32 quarter = (turn + 0x20000000u) >> 30;
+  const float y = (float)(int)(turn - (quarter << 30)) * 1.4629180792671596e-9f;  // 2 pi / 2^32
+  const float z = y * y;
+  float p = fmaf(z, 2.7557319e-6f, -1.9841270e-4f), q = fmaf(z, -2.7557319e-7f, 2.4801587e-5f);
+  p = fmaf(z, p, 8.3333333e-3f);
+  q = fmaf(z, q, -1.3888889e-3f);
+  p = fmaf(z, p, -1.6666667e-1f);
+  q = fmaf(z, q, 4.1666667e-2f);
+  q = fmaf(z, q, -0.5f);
+  const float sy = fmaf(y * z, p, y), cy = fmaf(z, q, 1.0f);
+  const float a = quarter & 1u ? cy : sy, b = quarter & 1u ? sy : cy;
+  *s = as_f(as_u(a) ^ ((quarter & 2u) << 30));
+  *c = as_f(as_u(b) ^ (((quarter + 1u) & 2u) << 30));
+}
+__device__ __forceinline__ i64 position_at(const RotaryArgs& a, i64 off) {
+  return a.pos64 ? static_cast<const i64*>(a.pos)[off] : (i64) static_cast<const int*>(a.pos)[off];
+}
+__device__ __forceinline__ double freq_at(const RotaryArgs& a, int f) {
+  return a.freq64 ? static_cast<const double*>(a.freq)[f] : (double)static_cast<const float*>(a.freq)[f];
+}
 // Sine and cosine of frequency f at a token; the identity behind the turned part.
 __device__ __forceinline__ void angle(const RotaryArgs& a, int f, i64 at_token, float* c, float* s) {
   *c = 1.0f;
   *s = 0.0f;
   if (f >= (a.R >> 1)) return;
-  const i64 off = (i64)a.axis_of[f] * a.ps[0] + at_token;
-  const double pos = a.pos64 ? (double)static_cast<const i64*>(a.pos)[off] : (double)static_cast<const int*>(a.pos)[off];
-  const double fr = a.freq64 ? static_cast<const double*>(a.freq)[f] : (double)static_cast<const float*>(a.freq)[f];
-  double turns = pos * fr * 0.15915494309189533577;  // 1 / (2 pi)
+  double turns = (double)position_at(a, (i64)a.axis_of[f] * a.ps[0] + at_token) * freq_at(a, f) * 0.15915494309189533577;  // 1 / (2 pi)
   turns -= rint(turns);
-  sincospif((float)(2.0 * turns), s, c);
+  turn_sincos((u32)__double2int_rn(turns * 4294967296.0), s, c);
+  if (!isfinite(turns)) *c = *s = as_f(0x7fffffffu);
   *s *= a.sign;
 }
 
@@ -177,7 +200,14 @@ __device__ __forceinline__ void store_pairs(T* row, i64 sd, int e0, int e1, int 
   }
 }
 
+// Sum over a row's lane group; LANES: how many where the kernel is made for it, 0: `lanes` of them.
+template <int LANES>
 __device__ __forceinline__ float group_sum(float v, int lanes) {
+  if constexpr (LANES > 0) {
+#pragma unroll
+    for (int o = LANES / 2; o; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
   if (lanes > 16) v += __shfl_xor_sync(0xffffffffu, v, 16);
   if (lanes > 8) v += __shfl_xor_sync(0xffffffffu, v, 8);
   if (lanes > 4) v += __shfl_xor_sync(0xffffffffu, v, 4);
@@ -270,7 +300,7 @@ struct Place {
 // of a CTA behind a barrier 63.9 us; no loop, one or two rows to a lane group 76 and 61 us (82 us where
 // the norm's weights add to what a CTA does first, 59.7 us here); the cosines of a token in registers
 // and rows two at a time 66 to 70 us; angles from 64-bit fractions of a turn instead of float64 65 us.
-template <class T, int V, int NS, bool NORM, bool ADJ>
+template <class T, int V, int NS, bool NORM, bool ADJ, int LANES>
 __global__ void __launch_bounds__(kRotThreads, V == 8 ? 5 : V > 1 ? 4 : 1) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   extern __shared__ __align__(16) float smem[];
   __shared__ i64 all_offs[kRotWarps][kRotMaxTile][4];  // token offsets of q, k, q_out, k_out
@@ -294,7 +324,7 @@ __global__ void __launch_bounds__(kRotThreads, V == 8 ? 5 : V > 1 ? 4 : 1) rotar
   }
   __syncwarp();
 
-  const int groups = 32 / a.lanes, p0 = lane & (a.lanes - 1);
+  const int lanes = LANES ? LANES : a.lanes, groups = 32 / lanes, p0 = lane & (lanes - 1);
   int e0[NS], e1[NS];
   bool has[NS];
 #pragma unroll
@@ -310,7 +340,7 @@ __global__ void __launch_bounds__(kRotThreads, V == 8 ? 5 : V > 1 ? 4 : 1) rotar
     x.load(static_cast<const T*>(a.x[z]) + (on ? offs[at.t][z] : 0) + (i64)(h - (z ? a.heads[0] : 0)) * a.xs[z][2], a.xs[z][3], e0, e1, has,
            a.D, on);
   };
-  Place at(lane / a.lanes, span);
+  Place at(lane / lanes, span);
   fetch(at);
   for (int t = 0; t < ntok; ++t) {
     i64 b, s;
@@ -355,7 +385,7 @@ __global__ void __launch_bounds__(kRotThreads, V == 8 ? 5 : V > 1 ? 4 : 1) rotar
         }
         ss += Lanes<V>::sum(s0) + Lanes<V>::sum(s1);
       }
-      const Wide<V> r = Lanes<V>::all(rsqrtf(fmaf(group_sum(ss, a.lanes), inv_d, a.eps)));
+      const Wide<V> r = Lanes<V>::all(rsqrtf(fmaf(group_sum<LANES>(ss, lanes), inv_d, a.eps)));
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         float f[V], g[V];
@@ -396,20 +426,37 @@ __global__ void __launch_bounds__(kRotThreads, V == 8 ? 5 : V > 1 ? 4 : 1) rotar
 }
 
 // Cosines and sines of the gradient's tokens: [tokens][2][slots V], quads of a slot as in shared memory.
+// A thread keeps its frequency, as a 64-bit fraction of a turn: positions are whole numbers, so the
+// product modulo 2^64 is the angle without its whole turns.
+constexpr int kRotTableTokens = 16;  // tokens of a thread
 template <int V>
 __global__ void __launch_bounds__(kRotThreads) rotary_table_kernel(const __grid_constant__ RotaryArgs a, float* table) {
-  const int row = a.slots * V;
-  const i64 i = (i64)blockIdx.x * kRotThreads + threadIdx.x;
-  const u32 tok = (u32)(i / row);
-  const int f = (int)(i - (i64)tok * row);
-  if (tok >= a.tokens) return;
-  i64 b, s;
-  token_place(a, tok, &b, &s);
-  float c, sn;
-  angle(a, f, b * a.ps[1] + s * a.ps[2], &c, &sn);
-  float* to = table + (i64)tok * 2 * row + spot<V>(f / V, f % V, a.slots);
-  to[0] = c;
-  to[row] = sn;
+  const int row = a.slots * V, f = blockIdx.y * blockDim.x + threadIdx.x;
+  if (f >= row) return;
+  const bool turned = f < (a.R >> 1);
+  u64 part = 0;
+  float nan = 0.0f;
+  if (turned) {
+    double turns = freq_at(a, f) * 0.15915494309189533577;  // 1 / (2 pi)
+    if (!isfinite(turns)) nan = as_f(0x7fffffffu);
+    turns -= floor(turns);
+    part = __double2ull_rn(turns * 18446744073709551616.0);
+  }
+  const i64 axis = turned ? (i64)a.axis_of[f] * a.ps[0] : 0;
+  const i64 first = ((i64)blockIdx.x * blockDim.y + threadIdx.y) * kRotTableTokens;
+  for (i64 tok = first; tok < min(first + kRotTableTokens, (i64)a.tokens); ++tok) {
+    float c = 1.0f, s = 0.0f;
+    if (turned) {
+      i64 b, q;
+      token_place(a, (u32)tok, &b, &q);
+      turn_sincos((u32)((part * (u64)position_at(a, axis + b * a.ps[1] + q * a.ps[2])) >> 32), &s, &c);
+      c += nan;
+      s = (s + nan) * a.sign;
+    }
+    float* to = table + tok * 2 * row + spot<V>(f / V, f % V, a.slots);
+    to[0] = c;
+    to[row] = s;
+  }
 }
 
 // Gradient of norm and rotation.  With n = x r, r = rsqrt(mean(x^2) + eps), g = dy rotated back and
@@ -420,7 +467,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_table_kernel(const __grid_
 // in a fixed order by rotary_weight_grad_kernel, so the gradient does not depend on scheduling.
 // The tables come from memory: formed here, between a warp's rows, they cost 40 of 140 us for 16384
 // tokens of 32 + 4 heads of 128.
-template <class T, int V, int NS, bool ADJ>
+template <class T, int V, int NS, bool ADJ, int LANES>
 __global__ void __launch_bounds__(kRotThreads, NS < 8 ? 2 : 1) rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
   extern __shared__ __align__(16) float smem[];
   const int row = a.slots * V, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -429,8 +476,8 @@ __global__ void __launch_bounds__(kRotThreads, NS < 8 ? 2 : 1) rotary_grad_kerne
   fill_weights<T, V>(a, z, w);
   __syncthreads();
 
-  const int group = lane / a.lanes, p0 = lane & (a.lanes - 1);
-  const int hp = a.step[z], tp = 32 / a.lanes / hp, tl = group / hp, hl = group & (hp - 1);
+  const int lanes = LANES ? LANES : a.lanes, group = lane / lanes, p0 = lane & (lanes - 1);
+  const int hp = a.step[z], tp = 32 / lanes / hp, tl = group / hp, hl = group & (hp - 1);
   const i64 sx = a.xs[z][2] * hp, sg = a.gs[z][2] * hp, sy = a.ys[z][2] * hp;
   const float inv_d = 1.0f / (float)a.D;
   int e0[NS], e1[NS];
@@ -443,37 +490,88 @@ __global__ void __launch_bounds__(kRotThreads, NS < 8 ? 2 : 1) rotary_grad_kerne
 #pragma unroll
     for (int j = 0; j < Lanes<V>::N; ++j) dwa[i].x[j] = dwb[i].x[j] = Lanes<V>::all(0.0f);
   }
-  // zero at first; later, where a group has no row, an earlier row of the same lanes and elements,
-  // which then counts times r = 0
-  Row<T, V, NS> xr, gr;
-  xr.clear();
-  gr.clear();
+  // A walk over this warp's rounds: the loads' walk is kRotStages rounds ahead of the other one.
+  struct Walk {
+    u32 tok;  // first of the round's tokens
+    int h0;
+  };
   const u32 step = (u32)a.ctas[z] * kRotWarps * (u32)tp;
-  u32 tok = ((blockIdx.x - (z ? (u32)a.ctas[0] : 0u)) * kRotWarps + warp) * (u32)tp;  // first of the round's tokens
-  int h0 = 0;
+  const u32 start = ((blockIdx.x - (z ? (u32)a.ctas[0] : 0u)) * kRotWarps + warp) * (u32)tp;
+  Walk ahead{start, 0}, at{start, 0};
   const T *px = nullptr, *pg = nullptr;
   T* py = nullptr;
   const float* tab = nullptr;
-  auto place = [&] {  // addresses of this group's token
-    const u32 t = min(tok + (u32)tl, a.tokens - 1);
+  auto place_in = [&] {  // addresses of this group's token
     i64 b, s;
-    token_place(a, t, &b, &s);
+    token_place(a, min(ahead.tok + (u32)tl, a.tokens - 1), &b, &s);
     px = static_cast<const T*>(a.x[z]) + b * a.xs[z][0] + s * a.xs[z][1] + hl * a.xs[z][2];
     pg = static_cast<const T*>(a.g[z]) + b * a.gs[z][0] + s * a.gs[z][1] + hl * a.gs[z][2];
+  };
+  auto place_out = [&] {
+    const u32 t = min(at.tok + (u32)tl, a.tokens - 1);
+    i64 b, s;
+    token_place(a, t, &b, &s);
     py = static_cast<T*>(a.y[z]) + b * a.ys[z][0] + s * a.ys[z][1] + hl * a.ys[z][2];
     tab = a.table + (i64)t * 2 * row;
   };
-  bool more = tok < a.tokens;
-  bool on = more && hl < H && tok + (u32)tl < a.tokens;
-  if (more) {
-    place();
-    xr.load(px, a.xs[z][3], e0, e1, has, a.D, on);
-    gr.load(pg, a.gs[z][3], e0, e1, has, a.D, on);
+  auto holds = [&](const Walk& w) { return w.tok < a.tokens && w.h0 + hl < H && w.tok + (u32)tl < a.tokens; };
+  // Rows on their way: in shared memory, every lane's vectors in its own places (no barrier, and no
+  // registers held); the element path reads into registers when it gets there.  Places are zero at
+  // first; where a group has no row they hold an earlier row of the same lanes and elements, which
+  // then counts times r = 0.
+  constexpr int S = V > 1 ? kRotStages : 1;
+  uint4* const ring = reinterpret_cast<uint4*>(w + 2 * row) + threadIdx.x;  // [S][4][threads]
+  Row<T, V, NS> xr, gr;
+  xr.clear();
+  gr.clear();
+  int stage_in = 0, stage_out = 0;
+  auto fetch = [&] {
+    const bool on = holds(ahead);
+    if constexpr (V > 1) {
+      if (on && has[0]) {
+        uint4* to = ring + stage_in * 4 * kRotThreads;
+        copy_async(to, px + e0[0]);
+        copy_async(to + kRotThreads, px + e1[0]);
+        copy_async(to + 2 * kRotThreads, pg + e0[0]);
+        copy_async(to + 3 * kRotThreads, pg + e1[0]);
+      }
+      copy_async_commit();
+      stage_in = stage_in + 1 == S ? 0 : stage_in + 1;
+    } else {
+      xr.load(px, a.xs[z][3], e0, e1, has, a.D, on);
+      gr.load(pg, a.gs[z][3], e0, e1, has, a.D, on);
+    }
+    if (ahead.tok >= a.tokens) return;
+    ahead.h0 += hp;
+    px += sx;
+    pg += sg;
+    if (ahead.h0 >= H) {
+      ahead.h0 = 0;
+      ahead.tok += step;
+      if (ahead.tok < a.tokens) place_in();
+    }
+  };
+  if (start < a.tokens) {
+    place_in();
+    place_out();
   }
-  while (more) {
-    T* const out = py;
-    const float* const c_row = tab;
-    const bool now = on;
+  if constexpr (V > 1) {
+#pragma unroll
+    for (int k = 0; k < 4 * S; ++k) ring[k * kRotThreads] = make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int k = 0; k < S; ++k) fetch();
+  while (at.tok < a.tokens) {
+    if constexpr (V > 1) {
+      copy_async_wait<S - 1>();
+      const uint4* from = ring + stage_out * 4 * kRotThreads;
+      xr.r[0].a = from[0];
+      xr.r[0].b = from[kRotThreads];
+      gr.r[0].a = from[2 * kRotThreads];
+      gr.r[0].b = from[3 * kRotThreads];
+      stage_out = stage_out + 1 == S ? 0 : stage_out + 1;
+    }
+    const bool now = holds(at);
     Lanes<V> xa[NS], xb[NS], ga[NS], gb[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
@@ -485,29 +583,15 @@ __global__ void __launch_bounds__(kRotThreads, NS < 8 ? 2 : 1) rotary_grad_kerne
       ga[i].set(f);
       gb[i].set(g);
     }
-    // the next round: further heads, or the next tokens
-    h0 += hp;
-    if (h0 < H) {
-      px += sx;
-      pg += sg;
-      py += sy;
-    } else {
-      h0 = 0;
-      tok += step;
-      more = tok < a.tokens;
-      if (more) place();
-    }
-    on = more && h0 + hl < H && tok + (u32)tl < a.tokens;
-    xr.load(px, a.xs[z][3], e0, e1, has, a.D, on);
-    gr.load(pg, a.gs[z][3], e0, e1, has, a.D, on);
+    fetch();
 
     float ss = 0.0f, hx = 0.0f;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       float c[V], sn[V], wa[V], wb[V];
       const int p = has[i] ? p0 + 32 * i : 0;
-      read_row<V>(c_row, p, a.slots, c);
-      read_row<V>(c_row + row, p, a.slots, sn);
+      read_row<V>(tab, p, a.slots, c);
+      read_row<V>(tab + row, p, a.slots, sn);
       read_row<V>(w, p, a.slots, wa);
       read_row<V>(w + row, p, a.slots, wb);
       Lanes<V> A, B, C, S;
@@ -515,22 +599,23 @@ __global__ void __launch_bounds__(kRotThreads, NS < 8 ? 2 : 1) rotary_grad_kerne
       B.set(wb);
       C.set(c);
       S.set(sn);
-      Wide<V> s0 = Lanes<V>::all(0.0f), s1 = s0, q0 = s0, q1 = s0;
+      Wide<V> s0, s1, q0, q1;
 #pragma unroll
       for (int j = 0; j < Lanes<V>::N; ++j) {
         const Wide<V> u = ga[i].x[j], v = gb[i].x[j];
         ga[i].x[j] = fma(u, C.x[j], mul(v, mul(S.x[j], Lanes<V>::all(-1.0f))));
         gb[i].x[j] = fma(v, C.x[j], mul(u, S.x[j]));
-        s0 = fma(xa[i].x[j], xa[i].x[j], s0);
-        s1 = fma(xb[i].x[j], xb[i].x[j], s1);
-        q0 = fma(mul(ga[i].x[j], xa[i].x[j]), A.x[j], q0);
-        q1 = fma(mul(gb[i].x[j], xb[i].x[j]), B.x[j], q1);
+        const Wide<V> g0 = mul(ga[i].x[j], xa[i].x[j]), g1 = mul(gb[i].x[j], xb[i].x[j]);
+        s0 = j ? fma(xa[i].x[j], xa[i].x[j], s0) : mul(xa[i].x[j], xa[i].x[j]);
+        s1 = j ? fma(xb[i].x[j], xb[i].x[j], s1) : mul(xb[i].x[j], xb[i].x[j]);
+        q0 = j ? fma(g0, A.x[j], q0) : mul(g0, A.x[j]);
+        q1 = j ? fma(g1, B.x[j], q1) : mul(g1, B.x[j]);
       }
       ss += Lanes<V>::sum(s0) + Lanes<V>::sum(s1);
       hx += Lanes<V>::sum(q0) + Lanes<V>::sum(q1);
     }
-    ss = group_sum(ss, a.lanes);
-    hx = group_sum(hx, a.lanes);
+    ss = group_sum<LANES>(ss, lanes);
+    hx = group_sum<LANES>(hx, lanes);
     const float r = now ? rsqrtf(fmaf(ss, inv_d, a.eps)) : 0.0f;
     const Wide<V> rr = Lanes<V>::all(r), kk = Lanes<V>::all(-(r * r * r) * (hx * inv_d));
 #pragma unroll
@@ -552,11 +637,20 @@ __global__ void __launch_bounds__(kRotThreads, NS < 8 ? 2 : 1) rotary_grad_kerne
       }
       A.get(f);
       B.get(g);
-      store_pairs<T, V, ADJ>(out, a.ys[z][3], e0[i], e1[i], a.D, now && has[i], f, g);
+      store_pairs<T, V, ADJ>(py, a.ys[z][3], e0[i], e1[i], a.D, now && has[i], f, g);
+    }
+    at.h0 += hp;
+    py += sy;
+    if (at.h0 >= H) {
+      at.h0 = 0;
+      at.tok += step;
+      if (at.tok < a.tokens) place_out();
     }
   }
+  if constexpr (V > 1) copy_async_wait<0>();
   if (!a.partial) return;
-  // lanes with the same slots in a warp, then the warps
+  // lanes with the same slots in a warp, then the warps (in the rows' place)
+  __syncthreads();
   float* red = w + 2 * row;  // [warps][2 * row]
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
@@ -566,11 +660,11 @@ __global__ void __launch_bounds__(kRotThreads, NS < 8 ? 2 : 1) rotary_grad_kerne
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float s0 = f[j], s1 = g[j];
-      for (int o = a.lanes; o < 32; o <<= 1) {
+      for (int o = lanes; o < 32; o <<= 1) {
         s0 += __shfl_xor_sync(0xffffffffu, s0, o);
         s1 += __shfl_xor_sync(0xffffffffu, s1, o);
       }
-      if (lane < a.lanes && has[i]) {
+      if (lane < lanes && has[i]) {
         red[warp * 2 * row + (p0 + 32 * i) * V + j] = s0;
         red[warp * 2 * row + row + (p0 + 32 * i) * V + j] = s1;
       }
@@ -686,6 +780,18 @@ static int slots_per_lane(const RotaryArgs& a) {
   return ns;
 }
 
+// Kernels whose lane groups are known when they are compiled, for the sizes of heads of 33 to 256
+// elements: without them every sum over a head tests which of five exchanges it takes part in.
+template <int V, class Fn>
+static void by_lanes(int lanes, Fn&& fn) {
+  if constexpr (V > 1) {
+    if (lanes == 4) return fn(std::integral_constant<int, 4>());
+    if (lanes == 8) return fn(std::integral_constant<int, 8>());
+    if (lanes == 16) return fn(std::integral_constant<int, 16>());
+  }
+  fn(std::integral_constant<int, 0>());
+}
+
 template <class T, int V, int NS, bool ADJ>
 static int launch_forward(RotaryArgs& a, bool norm, cudaStream_t s) {
   set_slots(&a, V);
@@ -701,8 +807,12 @@ static int launch_forward(RotaryArgs& a, bool norm, cudaStream_t s) {
   const int64_t units = ((int64_t)a.tokens + a.tile - 1) / a.tile * a.parts, grid = (units + kRotWarps - 1) / kRotWarps;
   TWG_REQUIRE(units + kRotWarps < (int64_t(1) << 32), "too many rows: %lld tokens of %d heads", (long long)a.tokens, H);
   const size_t smem = sizeof(float) * (size_t)row * (2 * a.tile * kRotWarps + (norm ? 4 : 0));
-  if (norm) rotary_kernel<T, V, NS, true, ADJ><<<(unsigned)grid, kRotThreads, smem, s>>>(a);
-  else rotary_kernel<T, V, NS, false, ADJ><<<(unsigned)grid, kRotThreads, smem, s>>>(a);
+  auto launch = [&](auto lanes) {
+    constexpr int LANES = decltype(lanes)::value;
+    if (norm) rotary_kernel<T, V, NS, true, ADJ, LANES><<<(unsigned)grid, kRotThreads, smem, s>>>(a);
+    else rotary_kernel<T, V, NS, false, ADJ, LANES><<<(unsigned)grid, kRotThreads, smem, s>>>(a);
+  };
+  by_lanes<V>(a.lanes, launch);
   TWG_CHECK_LAUNCH();
   g_last_path = V == 1 ? kPathStrided64 : kPathDense;
   return TWG_OK;
@@ -744,16 +854,30 @@ static int run_forward(const char* name, const TwgRotaryDesc* d, const void* q, 
   return dispatch_float(d->dtype, [&](auto* t) { return forward<std::remove_pointer_t<decltype(t)>>(a, vec, norm, s); });
 }
 
-// CTAs of q and of k in the gradient kernel, in proportion to their rows.  A function of the sizes
-// alone, so that the workspace can be sized without a device.
+// CTAs of q and of k in the gradient kernel, in proportion to what a token of each takes: its rounds, and
+// the addresses of a new token, which cost about kRotTokenCost rounds.  (Shares by rows alone left a tensor
+// of few heads, with a new token in every round, working for longer than the other: GRADOLD us in place of
+// GRADNEW for 16384 tokens of 32 + 4 heads of 128.)  A function of the sizes alone, so that the workspace
+// can be sized without a device.
+constexpr double kRotTokenCost = 2.0;
 static void grad_ctas(const TwgRotaryDesc* d, int* cq, int* ck) {
-  const int64_t tokens = d->batch * d->seq, hq = d->heads[0], hk = d->heads[1];
+  const int64_t tokens = d->batch * d->seq;
   *cq = *ck = 0;
-  if (tokens == 0 || hq + hk == 0) return;
-  const int64_t share = hq == 0 ? 0 : hk == 0 ? kRotGradCtas : std::min<int64_t>(std::max<int64_t>(kRotGradCtas * hq / (hq + hk), 1), kRotGradCtas - 1);
+  if (tokens == 0) return;
+  int groups = 32;
+  while (groups > 1 && 32 / groups * 32 < d->head_dim * float_size(d->dtype)) groups /= 2;
+  double cost[2] = {};
+  for (int t = 0; t < 2; ++t) {
+    int hp = 1;
+    while (hp < d->heads[t] && hp < groups) hp *= 2;
+    if (d->heads[t]) cost[t] = ((double)((d->heads[t] + hp - 1) / hp) + kRotTokenCost) * hp / groups;
+  }
+  if (cost[0] + cost[1] == 0.0) return;
+  int share = (int)(kRotGradCtas * cost[0] / (cost[0] + cost[1]) + 0.5);
+  if (cost[0] > 0.0 && cost[1] > 0.0) share = std::min(std::max(share, 1), kRotGradCtas - 1);
   const int64_t most = (tokens + kRotWarps - 1) / kRotWarps;  // a token to every warp
-  if (hq) *cq = (int)std::min<int64_t>(share, most);
-  if (hk) *ck = (int)std::min<int64_t>(kRotGradCtas - share, most);
+  if (cost[0] > 0.0) *cq = (int)std::min<int64_t>(share, most);
+  if (cost[1] > 0.0) *ck = (int)std::min<int64_t>(kRotGradCtas - share, most);
 }
 
 // The workspace: the CTAs' partial sums, then (on a 256-byte boundary) the tables.
@@ -771,13 +895,21 @@ static int launch_grad(RotaryArgs& a, float* table, cudaStream_t s) {
     a.step[t] = 1;
     while (a.step[t] < a.heads[t] && a.step[t] < 32 / a.lanes) a.step[t] *= 2;
   }
-  const int64_t grid = ((int64_t)a.tokens * row + kRotThreads - 1) / kRotThreads;
-  TWG_REQUIRE(grid <= 0x7fffffff, "too many tokens: %lld of %d frequencies", (long long)a.tokens, a.R / 2);
-  rotary_table_kernel<V><<<(unsigned)grid, kRotThreads, 0, s>>>(a, table);
+  int wide = 32;  // threads along the frequencies, the rest of a CTA along the tokens
+  while (wide < row && wide < kRotThreads) wide *= 2;
+  const int high = kRotThreads / wide, per = high * kRotTableTokens;
+  rotary_table_kernel<V><<<dim3((a.tokens + per - 1) / per, (row + wide - 1) / wide), dim3(wide, high), 0, s>>>(a, table);
   TWG_CHECK_LAUNCH();
   a.table = table;
-  const size_t smem = sizeof(float) * (size_t)row * (2 + 2 * kRotWarps);
-  rotary_grad_kernel<T, V, NS, ADJ><<<a.ctas[0] + a.ctas[1], kRotThreads, smem, s>>>(a);
+  const size_t smem = sizeof(float) * (size_t)row * 2 + std::max(sizeof(float) * (size_t)row * 2 * kRotWarps,
+                                                                 V > 1 ? sizeof(uint4) * 4 * kRotStages * kRotThreads : (size_t)0);
+  cudaError_t err = cudaSuccess;
+  by_lanes<V>(a.lanes, [&](auto lanes) {
+    const auto kernel = rotary_grad_kernel<T, V, NS, ADJ, decltype(lanes)::value>;
+    if (smem > 48 * 1024) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err == cudaSuccess) kernel<<<a.ctas[0] + a.ctas[1], kRotThreads, smem, s>>>(a);
+  });
+  TWG_CUDA(err);
   TWG_CHECK_LAUNCH();
   g_last_path = V == 1 ? kPathStrided64 : kPathDense;
   return TWG_OK;

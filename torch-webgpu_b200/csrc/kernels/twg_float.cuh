@@ -66,6 +66,17 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8], const __nv_bfloat16*)
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// 16 bytes of global memory to shared memory, on their way until a wait: copy_async_wait<N> returns when
+// at most the calling thread's N latest commits are still under way.
+__device__ __forceinline__ void copy_async(uint4* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((u32)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Two float32 values in one register pair, and arithmetic on both in one instruction.
 struct Two {
   u64 v;

@@ -9,7 +9,7 @@
 // dy and writes dx), about ten instructions per element in between.  One row is one head of one
 // token.  A group of lanes owns a row, each lane two 16-byte vectors that hold both partners of
 // its pairs, so a row is in registers between its load and its store and the norm's sum is a few
-// shuffles.  The angle is the only part that needs more than 32 bits (a position of 10^6 leaves
+// shuffles (heads that 16 bytes do not divide take vectors of 8 or 4, or single elements).  The angle is the only part that needs more than 32 bits (a position of 10^6 leaves
 // 2^-4 of a turn in float32): it is formed in 64-bit fractions of a turn, once per token and
 // frequency, and its sine and cosine wait in shared memory for every head of the token.
 #include "twg_float.cuh"
@@ -53,7 +53,7 @@ struct RotaryArgs {
 // the slots, so that the 16-byte reads of a group's lanes hit different banks.
 template <int V>
 __device__ __forceinline__ int spot(int p, int j, int slots) {
-  if constexpr (V == 1) return p;
+  if constexpr (V <= 2) return p * V + j;
   else return ((j >> 2) * slots + p) * 4 + (j & 3);
 }
 // First elements of the two vectors of slot p.
@@ -135,7 +135,10 @@ __device__ __forceinline__ void fill_weights(const RotaryArgs& a, int tensor, fl
 template <int V>
 __device__ __forceinline__ void read_row(const float* tab, int p, int slots, float (&out)[V]) {
   if constexpr (V == 1) out[0] = tab[p];
-  else {
+  else if constexpr (V == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(tab + 2 * p);
+    out[0] = v.x; out[1] = v.y;
+  } else {
 #pragma unroll
     for (int q = 0; q < V / 4; ++q) {
       const float4 v = *reinterpret_cast<const float4*>(tab + (q * slots + p) * 4);
@@ -147,7 +150,7 @@ __device__ __forceinline__ void read_row(const float* tab, int p, int slots, flo
 // Raw contents of the two vectors of a lane's slot (or its two elements on the scalar path).
 template <class T, int V>
 struct Raw {
-  uint4 a, b;
+  typename VecBytes<V * (int)sizeof(T)>::type a, b;
 };
 template <class T>
 struct Raw<T, 1> {
@@ -179,7 +182,7 @@ __device__ __forceinline__ void store_pairs(T* row, i64 sd, int e0, int e1, int 
     row[e0 * sd] = from_f32<T>(a[0]);
     if (e1 < D) row[e1 * sd] = from_f32<T>(b[0]);
   } else {
-    uint4 x, y;
+    typename VecBytes<V * (int)sizeof(T)>::type x, y;
     if constexpr (!ADJ) {
       x = pack(a, static_cast<const T*>(nullptr));
       y = pack(b, static_cast<const T*>(nullptr));
@@ -194,8 +197,8 @@ __device__ __forceinline__ void store_pairs(T* row, i64 sd, int e0, int e1, int 
       y = pack(v, static_cast<const T*>(nullptr));
     }
     if (on) {
-      st_v4(row + e0, x);
-      st_v4(row + e1, y);
+      st_vec(row + e0, x);
+      st_vec(row + e1, y);
     }
   }
 }
@@ -261,7 +264,7 @@ struct Row {
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       if constexpr (V == 1) r[i].a = r[i].b = 0.0f;
-      else r[i].a = r[i].b = make_uint4(0, 0, 0, 0);
+      else r[i].a = r[i].b = decltype(r[i].a){};
     }
   }
   __device__ __forceinline__ void load(const T* row, i64 sd, const int (&e0)[NS], const int (&e1)[NS], const bool (&has)[NS], int D, bool on) {
@@ -273,8 +276,8 @@ struct Row {
         r[i].a = to_f32(row[e0[i] * sd]);
         if (e1[i] < D) r[i].b = to_f32(row[e1[i] * sd]);
       } else {
-        r[i].a = ld_v4(row + e0[i]);
-        r[i].b = ld_v4(row + e1[i]);
+        ld_vec(r[i].a, row + e0[i]);
+        ld_vec(r[i].b, row + e1[i]);
       }
     }
   }
@@ -520,7 +523,8 @@ __global__ void __launch_bounds__(kRotThreads, NS < 8 ? 2 : 1) rotary_grad_kerne
   // first; where a group has no row they hold an earlier row of the same lanes and elements, which
   // then counts times r = 0.
   constexpr int S = V > 1 ? kRotStages : 1;
-  uint4* const ring = reinterpret_cast<uint4*>(w + 2 * row) + threadIdx.x;  // [S][4][threads]
+  using Vec = std::remove_reference_t<decltype(Raw<T, V>::a)>;
+  Vec* const ring = reinterpret_cast<Vec*>(w + 2 * row) + threadIdx.x;  // [S][4][threads]
   Row<T, V, NS> xr, gr;
   xr.clear();
   gr.clear();
@@ -529,7 +533,7 @@ __global__ void __launch_bounds__(kRotThreads, NS < 8 ? 2 : 1) rotary_grad_kerne
     const bool on = holds(ahead);
     if constexpr (V > 1) {
       if (on && has[0]) {
-        uint4* to = ring + stage_in * 4 * kRotThreads;
+        Vec* to = ring + stage_in * 4 * kRotThreads;
         copy_async(to, px + e0[0]);
         copy_async(to + kRotThreads, px + e1[0]);
         copy_async(to + 2 * kRotThreads, pg + e0[0]);
@@ -557,14 +561,14 @@ __global__ void __launch_bounds__(kRotThreads, NS < 8 ? 2 : 1) rotary_grad_kerne
   }
   if constexpr (V > 1) {
 #pragma unroll
-    for (int k = 0; k < 4 * S; ++k) ring[k * kRotThreads] = make_uint4(0, 0, 0, 0);
+    for (int k = 0; k < 4 * S; ++k) ring[k * kRotThreads] = Vec{};
   }
 #pragma unroll
   for (int k = 0; k < S; ++k) fetch();
   while (at.tok < a.tokens) {
     if constexpr (V > 1) {
       copy_async_wait<S - 1>();
-      const uint4* from = ring + stage_out * 4 * kRotThreads;
+      const Vec* from = ring + stage_out * 4 * kRotThreads;
       xr.r[0].a = from[0];
       xr.r[0].b = from[kRotThreads];
       gr.r[0].a = from[2 * kRotThreads];
@@ -729,10 +733,8 @@ static int check_rotary(const char* name, const TwgRotaryDesc* d) {
   return TWG_OK;
 }
 
-// Fills everything but the pointers that only one direction has; *vec says whether every row can be
-// read and written as 16-byte vectors whose lanes hold both partners of their pairs.
-static void fill_rotary(const TwgRotaryDesc* d, bool grad, RotaryArgs* a, bool* vec) {
-  const int V = 16 / float_size(d->dtype);
+// Fills everything but the pointers.
+static void fill_rotary(const TwgRotaryDesc* d, RotaryArgs* a) {
   memset(a, 0, sizeof(*a));
   memcpy(a->xs, d->in_strides, sizeof(a->xs));
   memcpy(a->ys, d->out_strides, sizeof(a->ys));
@@ -749,24 +751,26 @@ static void fill_rotary(const TwgRotaryDesc* d, bool grad, RotaryArgs* a, bool* 
   a->freq64 = d->freq_dtype == TWG_DTYPE_F64;
   a->w32 = d->weight_dtype == TWG_DTYPE_F32;
   a->adjacent = d->adjacent != 0;
-  bool ok = a->D % (2 * V) == 0 && a->D / (2 * V) <= 32 && (a->adjacent || (a->R / 2) % V == 0);
-  const int64_t size[3] = {d->batch, d->seq, 0};
-  for (int t = 0; t < 2 && ok; ++t) {
-    if (a->heads[t] == 0) continue;
-    for (int k = 0; k < 3; ++k) {
-      if ((k < 2 ? size[k] : d->heads[t]) <= 1) continue;
-      ok = ok && a->xs[t][k] % V == 0 && a->ys[t][k] % V == 0 && (!grad || a->gs[t][k] % V == 0);
-    }
-    ok = ok && a->xs[t][3] == 1 && a->ys[t][3] == 1 && (!grad || a->gs[t][3] == 1);
-  }
-  *vec = ok;
 }
-static bool rows_aligned(const RotaryArgs& a, bool grad) {
-  for (int t = 0; t < 2; ++t) {
-    if (a.heads[t] == 0) continue;
-    if (!is_aligned(a.x[t], 16) || !is_aligned(a.y[t], 16) || (grad && !is_aligned(a.g[t], 16))) return false;
+// Elements of the widest vectors in which every row can be read and written, with both partners of
+// their pairs in one lane: 16 bytes, or 8 or 4 where sizes, strides or addresses ask for it; 1: none.
+static int vector_width(const TwgRotaryDesc* d, const RotaryArgs& a, bool grad) {
+  const int size = float_size(d->dtype);
+  const int64_t extent[2] = {d->batch, d->seq};
+  for (int V = 16 / size; V >= 2; V /= 2) {
+    bool ok = a.D % (2 * V) == 0 && a.D / (2 * V) <= 32 && (a.adjacent || (a.R / 2) % V == 0);
+    for (int t = 0; t < 2 && ok; ++t) {
+      if (a.heads[t] == 0) continue;
+      for (int k = 0; k < 3; ++k) {
+        if ((k < 2 ? extent[k] : d->heads[t]) <= 1) continue;
+        ok = ok && a.xs[t][k] % V == 0 && a.ys[t][k] % V == 0 && (!grad || a.gs[t][k] % V == 0);
+      }
+      ok = ok && a.xs[t][3] == 1 && a.ys[t][3] == 1 && (!grad || a.gs[t][3] == 1);
+      ok = ok && is_aligned(a.x[t], V * size) && is_aligned(a.y[t], V * size) && (!grad || is_aligned(a.g[t], V * size));
+    }
+    if (ok) return V;
   }
-  return true;
+  return 1;
 }
 // Slots of a row and lanes of its group.
 static void set_slots(RotaryArgs* a, int V) {
@@ -782,9 +786,9 @@ static int slots_per_lane(const RotaryArgs& a) {
 
 // Kernels whose lane groups are known when they are compiled, for the sizes of heads of 33 to 256
 // elements: without them every sum over a head tests which of five exchanges it takes part in.
-template <int V, class Fn>
+template <bool WIDE, class Fn>
 static void by_lanes(int lanes, Fn&& fn) {
-  if constexpr (V > 1) {
+  if constexpr (WIDE) {
     if (lanes == 4) return fn(std::integral_constant<int, 4>());
     if (lanes == 8) return fn(std::integral_constant<int, 8>());
     if (lanes == 16) return fn(std::integral_constant<int, 16>());
@@ -812,15 +816,22 @@ static int launch_forward(RotaryArgs& a, bool norm, cudaStream_t s) {
     if (norm) rotary_kernel<T, V, NS, true, ADJ, LANES><<<(unsigned)grid, kRotThreads, smem, s>>>(a);
     else rotary_kernel<T, V, NS, false, ADJ, LANES><<<(unsigned)grid, kRotThreads, smem, s>>>(a);
   };
-  by_lanes<V>(a.lanes, launch);
+  by_lanes<V == kVecOf<T>>(a.lanes, launch);
   TWG_CHECK_LAUNCH();
   g_last_path = V == 1 ? kPathStrided64 : kPathDense;
   return TWG_OK;
 }
 template <class T>
-static int forward(RotaryArgs& a, bool vec, bool norm, cudaStream_t s) {
-  constexpr int V = kVecOf<T>;
-  if (vec) return a.adjacent ? launch_forward<T, V, 1, true>(a, norm, s) : launch_forward<T, V, 1, false>(a, norm, s);
+static int forward(RotaryArgs& a, int V, bool norm, cudaStream_t s) {
+  auto wide = [&](auto v) {
+    constexpr int W = decltype(v)::value;
+    return a.adjacent ? launch_forward<T, W, 1, true>(a, norm, s) : launch_forward<T, W, 1, false>(a, norm, s);
+  };
+  if (V == 2) return wide(std::integral_constant<int, 2>());
+  if (V == 4) return wide(std::integral_constant<int, 4>());
+  if constexpr (kVecOf<T> == 8) {
+    if (V == 8) return wide(std::integral_constant<int, 8>());
+  }
   set_slots(&a, 1);
   switch (slots_per_lane(a)) {
     case 1: return launch_forward<T, 1, 1, false>(a, norm, s);
@@ -835,8 +846,7 @@ static int run_forward(const char* name, const TwgRotaryDesc* d, const void* q, 
   g_last_path = kPathNone;
   if (int rc = check_rotary(name, d)) return rc;
   RotaryArgs a;
-  bool vec;
-  fill_rotary(d, false, &a, &vec);
+  fill_rotary(d, &a);
   if (a.tokens == 0 || a.heads[0] + a.heads[1] == 0) return TWG_OK;
   TWG_REQUIRE(positions && inv_freq, "%s: positions or inv_freq is null", name);
   TWG_REQUIRE(a.heads[0] == 0 || (q && q_out), "%s: q or its output is null", name);
@@ -849,9 +859,9 @@ static int run_forward(const char* name, const TwgRotaryDesc* d, const void* q, 
   a.pos = positions;
   a.freq = inv_freq;
   a.sign = d->inverse ? -1.0f : 1.0f;
-  vec = vec && rows_aligned(a, false);
+  const int V = vector_width(d, a, false);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dispatch_float(d->dtype, [&](auto* t) { return forward<std::remove_pointer_t<decltype(t)>>(a, vec, norm, s); });
+  return dispatch_float(d->dtype, [&](auto* t) { return forward<std::remove_pointer_t<decltype(t)>>(a, V, norm, s); });
 }
 
 // CTAs of q and of k in the gradient kernel, in proportion to what a token of each takes: its rounds, and
@@ -902,9 +912,9 @@ static int launch_grad(RotaryArgs& a, float* table, cudaStream_t s) {
   TWG_CHECK_LAUNCH();
   a.table = table;
   const size_t smem = sizeof(float) * (size_t)row * 2 + std::max(sizeof(float) * (size_t)row * 2 * kRotWarps,
-                                                                 V > 1 ? sizeof(uint4) * 4 * kRotStages * kRotThreads : (size_t)0);
+                                                                 V > 1 ? sizeof(T) * V * 4 * kRotStages * kRotThreads : (size_t)0);
   cudaError_t err = cudaSuccess;
-  by_lanes<V>(a.lanes, [&](auto lanes) {
+  by_lanes<V == kVecOf<T>>(a.lanes, [&](auto lanes) {
     const auto kernel = rotary_grad_kernel<T, V, NS, ADJ, decltype(lanes)::value>;
     if (smem > 48 * 1024) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (err == cudaSuccess) kernel<<<a.ctas[0] + a.ctas[1], kRotThreads, smem, s>>>(a);
@@ -915,9 +925,16 @@ static int launch_grad(RotaryArgs& a, float* table, cudaStream_t s) {
   return TWG_OK;
 }
 template <class T>
-static int backward(RotaryArgs& a, bool vec, float* table, cudaStream_t s) {
-  constexpr int V = kVecOf<T>;
-  if (vec) return a.adjacent ? launch_grad<T, V, 1, true>(a, table, s) : launch_grad<T, V, 1, false>(a, table, s);
+static int backward(RotaryArgs& a, int V, float* table, cudaStream_t s) {
+  auto wide = [&](auto v) {
+    constexpr int W = decltype(v)::value;
+    return a.adjacent ? launch_grad<T, W, 1, true>(a, table, s) : launch_grad<T, W, 1, false>(a, table, s);
+  };
+  if (V == 2) return wide(std::integral_constant<int, 2>());
+  if (V == 4) return wide(std::integral_constant<int, 4>());
+  if constexpr (kVecOf<T> == 8) {
+    if (V == 8) return wide(std::integral_constant<int, 8>());
+  }
   set_slots(&a, 1);
   switch (slots_per_lane(a)) {
     case 1: return launch_grad<T, 1, 1, false>(a, table, s);
@@ -959,8 +976,7 @@ extern "C" int twg_qk_norm_rotary_backward(const TwgRotaryDesc* d, const void* q
   if (int rc = check_rotary(name, d)) return rc;
   TWG_REQUIRE(!d->inverse, "%s: inverse belongs to twg_rotary", name);
   RotaryArgs a;
-  bool vec;
-  fill_rotary(d, true, &a, &vec);
+  fill_rotary(d, &a);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   grad_ctas(d, &a.ctas[0], &a.ctas[1]);
   const bool any = a.ctas[0] + a.ctas[1] > 0;
@@ -983,8 +999,8 @@ extern "C" int twg_qk_norm_rotary_backward(const TwgRotaryDesc* d, const void* q
     a.freq = inv_freq;
     a.sign = -1.0f;
     a.partial = sums ? static_cast<float*>(workspace) : nullptr;
-    vec = vec && rows_aligned(a, true);
-    const int rc = dispatch_float(d->dtype, [&](auto* t) { return backward<std::remove_pointer_t<decltype(t)>>(a, vec, table, s); });
+    const int V = vector_width(d, a, true);
+    const int rc = dispatch_float(d->dtype, [&](auto* t) { return backward<std::remove_pointer_t<decltype(t)>>(a, V, table, s); });
     if (rc != TWG_OK) return rc;
   }
   if (!sums) return TWG_OK;

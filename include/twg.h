@@ -132,7 +132,6 @@ int twg_memcpy_d2d(void* dst_dev, const void* src_dev, size_t nbytes, void* stre
 int twg_memset(void* dst_dev, int value, size_t nbytes, void* stream);
 int twg_host_alloc_pinned(void** ptr, size_t nbytes);
 int twg_host_free_pinned(void* ptr);
-int twg_host_is_pinned(const void* ptr, int* pinned);   /* host memory the device reads directly, whoever allocated it */
 /* Strided / broadcasting device copy of `itemsize`-byte elements (1, 2, 4, 8 or 16).
  * Replaces unary_kernel<UnaryOp::Copy> (csrc/ops/copy.cpp:123-134, unary.cpp:88).
  * desc operands: [0] = out, [1] = in. */

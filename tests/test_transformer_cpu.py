@@ -206,6 +206,28 @@ def test_op_refusals_without_a_device():
             call()
 
 
+def test_shapes_of_symbols():
+    """A graph traced for any batch: result shapes follow the symbols."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    seen = []
+
+    def step(q, k, pos, f, logits, tokens):
+        seen.append(type(q.shape[0]).__name__)
+        out = ops.qk_norm_rotary(q, k, None, None, pos, f)
+        back = ops.qk_norm_rotary_backward(*out, q, k, None, None, pos, f)
+        turned = ops.rotary_qk(q, k, pos, f)
+        o = ops.token_logprobs(logits, tokens, top=3)
+        dx = ops.token_logprobs_backward(o[0], None, None, logits, tokens, o[1], o[2])
+        return [*out, *back, *turned, ops.dropout(q, 0.5, 1), *o, dx]
+
+    args = (meta(3, 5, 8, 64), meta(3, 5, 2, 64), meta(3, 5, dtype=torch.long), meta(32), meta(7, 100), meta(7, dtype=torch.long))
+    gm = make_fx(step, tracing_mode="symbolic")(*args)
+    assert seen == ["SymInt"]
+    values = [tuple(int(s) for s in n.meta["val"].shape) for n in next(iter(reversed(gm.graph.nodes))).args[0]]
+    q, k = (3, 5, 8, 64), (3, 5, 2, 64)
+    assert values == [q, k, q, k, (0,), (0,), q, k, q, (7,), (7,), (7,), (7, 3), (7, 3), (7, 100)]
+
+
 def test_generator_state_of_the_device_module():
     before = torch.webgpu.get_rng_state()
     torch.manual_seed(99)

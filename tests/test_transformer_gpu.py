@@ -655,6 +655,63 @@ def test_ops_run_on_the_current_stream():
     R.assert_within(got[6], R.turn(x.view(256, 16, 128).double(), ang, False), R.TURN * R.pair_size(x.view(256, 16, 128).double(), 128, False), "rotated")
 
 
+def test_backward_follows_the_forward_stream():
+    """The gradient runs on the stream of the forward pass, wherever backward() is called from; two host
+    threads may run the ops at once."""
+    import threading
+    b, s, h, d = 2, 64, 4, 64
+    f, pos = freqs(d).to("webgpu"), torch.arange(s).expand(b, s).to("webgpu")
+    torch.webgpu.synchronize()
+    ang = R.angles(torch.arange(s).expand(b, s)[None], freqs(d), [0] * (d // 2), (b, s))
+    failures = []
+
+    def work(seed):
+        try:
+            q, k, gq, gk = (rand(b, s, h, d, seed=seed + i) for i in range(4))
+            side = torch.Stream(device="webgpu")
+            for _ in range(5):
+                with side:
+                    leaves = [t.to("webgpu").requires_grad_() for t in (q, k)]
+                    out = ops.qk_norm_rotary(*leaves, None, None, pos, f)
+                    g = [t.to("webgpu") for t in (gq, gk)]
+                side.synchronize()
+                torch.autograd.backward(out, g)
+                torch.webgpu.synchronize()
+                for leaf, x, gr in zip(leaves, (q, k), (gq, gk)):
+                    _, _, dx, dxb, _, _ = norm_reference(x, None, gr, ang, d, False, float(np.float32(1e-6)))
+                    R.assert_within(leaf.grad, dx, dxb, "dx")
+        except BaseException as e:  # noqa: BLE001 - reported by the main thread
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(100 * i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures[0]
+
+
+def test_no_gradient_for_frequencies():
+    f = freqs(64).to("webgpu").requires_grad_()
+    x, pos = rand(3, 2, 64).to("webgpu"), torch.arange(3).to("webgpu")
+    with pytest.raises(RuntimeError, match="no gradient for inv_freq"):
+        ops.rotary(x, pos, f)
+    with torch.no_grad():
+        assert ops.rotary(x, pos, f).shape == x.shape
+
+
+def test_compiled_function_of_any_batch():
+    from torch_webgpu import webgpu_backend
+
+    def step(logits, tokens, state):
+        return torch.ops.webgpu.token_logprobs(torch.ops.webgpu.dropout_state(logits, 0.1, state), tokens)[0]
+
+    fn = torch.compile(step, backend=webgpu_backend, dynamic=True)
+    for n in (3, 5, 8):
+        args = [t.to("webgpu") for t in (rand(n, 70), torch.arange(n), torch.tensor([1, 2]))]
+        assert torch.equal(fn(*args).cpu(), step(*args).cpu())
+
+
 def test_graphs_replay_with_new_inputs_and_a_shared_workspace(abi):
     """Two captured graphs that share the gradient's workspace, replayed in turn on new contents; dropout
     draws another mask in every replay through its state."""

@@ -198,10 +198,6 @@ struct WebGPUHooks final : public at::PrivateUse1HooksInterface {
   bool isAvailable() const override { return count() > 0; }
   bool hasPrimaryContext(c10::DeviceIndex index) const override { return index >= 0 && index < count(); }
   c10::DeviceIndex deviceCount() const override { return count(); }
-  bool isPinnedPtr(const void* data) const override {
-    int pinned = 0;
-    return twg_host_is_pinned(data, &pinned) == TWG_OK && pinned != 0;
-  }
   c10::DeviceIndex getCurrentDevice() const override { return current_device(); }
   void setCurrentDevice(c10::DeviceIndex index) const override { set_current_device(index); }
   c10::DeviceIndex exchangeDevice(c10::DeviceIndex index) const override {

@@ -44,6 +44,9 @@ static c10::DeviceIndex tensor_device(const at::Tensor& t) {
   return t.device().index() < 0 ? core::current_device() : t.device().index();
 }
 
+// Shapes of a traced graph may be symbols; the checks then wait for the call with the sizes themselves.
+static bool symbolic(const at::Tensor& t) { return t.unsafeGetTensorImpl()->has_symbolic_sizes_strides(); }
+
 // ---- rotation, and the norm of queries and keys in front of it -----------------------------
 // q and k: [batch, seq, heads, dim] or [tokens, heads, dim].
 static void put_strides(int64_t (&out)[4], const at::Tensor& t) {
@@ -149,6 +152,7 @@ static void set_weight_dtype(const char* name, TwgRotaryDesc& d, const OptTensor
 
 static std::tuple<at::Tensor, at::Tensor> run_rotary(const char* name, const at::Tensor& q, const at::Tensor* k, const at::Tensor& positions,
                                                      const at::Tensor& inv_freq, c10::IntArrayRef axis_of, bool adjacent, bool inverse) {
+  if (symbolic(q) || (k && symbolic(*k)) || symbolic(positions)) return {at::empty_like(q), k ? at::empty_like(*k) : at::Tensor()};
   Rotary r = describe_rotary(name, q, k, positions, inv_freq, axis_of, adjacent);
   at::Tensor qo = at::empty_like(q), ko;
   if (k) ko = at::empty_like(*k);
@@ -175,6 +179,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rotary(const at::Tensor& q, const at:
                                                   const at::Tensor& positions, const at::Tensor& inv_freq, c10::IntArrayRef axis_of, double eps,
                                                   bool adjacent) {
   const char* name = "qk_norm_rotary";
+  if (symbolic(q) || symbolic(k) || symbolic(positions)) return {at::empty_like(q), at::empty_like(k)};
   Rotary r = describe_rotary(name, q, &k, positions, inv_freq, axis_of, adjacent);
   TORCH_CHECK(eps >= 0, "torch_webgpu: qk_norm_rotary: eps must not be negative");
   check_weight(name, q, q_weight);
@@ -199,6 +204,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rotary_backwa
     const at::Tensor& dq_out, const at::Tensor& dk_out, const at::Tensor& q, const at::Tensor& k, const OptTensor& q_weight,
     const OptTensor& k_weight, const at::Tensor& positions, const at::Tensor& inv_freq, c10::IntArrayRef axis_of, double eps, bool adjacent) {
   const char* name = "qk_norm_rotary_backward";
+  if (symbolic(q) || symbolic(k) || symbolic(positions)) {
+    auto like = [&](const OptTensor& w) { return given(w) ? at::empty_like(*w) : at::empty({0}, q.options()); };
+    return {at::empty_like(q), at::empty_like(k), like(q_weight), like(k_weight)};
+  }
   Rotary r = describe_rotary(name, q, &k, positions, inv_freq, axis_of, adjacent);
   TORCH_CHECK(eps >= 0, "torch_webgpu: qk_norm_rotary_backward: eps must not be negative");
   check_weight(name, q, q_weight);
@@ -233,6 +242,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rotary_backwa
 
 // ---- dropout -----------------------------------------------------------------------------------
 static at::Tensor run_dropout(const at::Tensor& x, double p, uint64_t seed, int64_t offset, const at::Tensor* state, const OptTensor& residual) {
+  if (symbolic(x)) return at::empty_like(x);
   const int dtype = dtype_of("dropout", x);
   TORCH_CHECK(p >= 0 && p <= 1, "dropout probability has to be between 0 and 1, but got ", p);
   TORCH_CHECK(x.dim() <= TWG_MAX_DIMS, "torch_webgpu: dropout supports at most ", TWG_MAX_DIMS, " dimensions, got ", x.dim());
@@ -317,8 +327,15 @@ static Logprobs describe_logprobs(const char* name, const at::Tensor& logits, co
 using LogprobsOut = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
 
 LogprobsOut token_logprobs(const at::Tensor& logits, const at::Tensor& tokens, int64_t top, double scale) {
-  Logprobs r = describe_logprobs("token_logprobs", logits, tokens, top, scale);
   const auto numbers = logits.options().dtype(at::kFloat);
+  if (symbolic(logits) || symbolic(tokens)) {
+    const auto lead = logits.sym_sizes().slice(0, logits.dim() - 1);
+    std::vector<c10::SymInt> tops(lead.begin(), lead.end());
+    tops.emplace_back(top);
+    return {at::empty_symint(tokens.sym_sizes(), numbers), at::empty_symint(lead, numbers), at::empty_symint(lead, numbers),
+            at::empty_symint(tops, numbers), at::empty_symint(tops, logits.options().dtype(at::kLong))};
+  }
+  Logprobs r = describe_logprobs("token_logprobs", logits, tokens, top, scale);
   at::Tensor logp = at::empty(tokens.sizes(), numbers), entropy = at::empty(r.lead, numbers), lse = at::empty(r.lead, numbers);
   std::vector<int64_t> tops = r.lead;
   tops.push_back(top);
@@ -336,6 +353,7 @@ LogprobsOut token_logprobs(const at::Tensor& logits, const at::Tensor& tokens, i
 at::Tensor token_logprobs_backward(const OptTensor& dlogp, const OptTensor& dentropy, const OptTensor& dlse, const at::Tensor& logits,
                                    const at::Tensor& tokens, const at::Tensor& entropy, const at::Tensor& lse, double scale) {
   const char* name = "token_logprobs_backward";
+  if (symbolic(logits) || symbolic(tokens)) return at::empty_symint(logits.sym_sizes(), logits.options());
   Logprobs r = describe_logprobs(name, logits, tokens, 0, scale);
   auto dense = [&](const OptTensor& g, c10::IntArrayRef shape) -> at::Tensor {
     if (!given(g)) return at::Tensor();
@@ -411,12 +429,17 @@ struct RotaryQkGrad : public Function<RotaryQkGrad> {
     return {dq, dk, {}, {}, {}, {}, {}};
   }
 };
+static void no_gradient(const char* name, const at::Tensor& inv_freq) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && inv_freq.requires_grad()), "torch_webgpu: ", name, " has no gradient for inv_freq");
+}
 at::Tensor rotary_autograd(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& inv_freq, c10::IntArrayRef axis_of, bool adjacent,
                            bool inverse) {
+  no_gradient("rotary", inv_freq);
   return RotaryGrad::apply(x, positions, inv_freq, axis_of.vec(), adjacent, inverse);
 }
 std::tuple<at::Tensor, at::Tensor> rotary_qk_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
                                                       const at::Tensor& inv_freq, c10::IntArrayRef axis_of, bool adjacent, bool inverse) {
+  no_gradient("rotary_qk", inv_freq);
   auto out = RotaryQkGrad::apply(q, k, positions, inv_freq, axis_of.vec(), adjacent, inverse);
   return {out[0], out[1]};
 }
@@ -443,6 +466,7 @@ struct QkNormGrad : public Function<QkNormGrad> {
 std::tuple<at::Tensor, at::Tensor> qk_norm_rotary_autograd(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, const OptTensor& kw,
                                                            const at::Tensor& positions, const at::Tensor& inv_freq, c10::IntArrayRef axis_of,
                                                            double eps, bool adjacent) {
+  no_gradient("qk_norm_rotary", inv_freq);
   auto out = QkNormGrad::apply(q, k, qw, kw, positions, inv_freq, axis_of.vec(), eps, adjacent);
   return {out[0], out[1]};
 }

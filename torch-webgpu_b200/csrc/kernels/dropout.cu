@@ -92,9 +92,10 @@ __device__ __forceinline__ void load_state(const DropoutArgs& a, u64* seed, u64*
   *seed = a.state ? a.state[0] : a.seed;
   *offset = a.state ? a.state[1] + a.offset : a.offset;
 }
-// A dropped element is zero whatever x holds there, NaN and infinities included.
-__device__ __forceinline__ float drop(const DropoutArgs& a, u32 word, float x) {
-  return word >= a.threshold && !a.drop_all ? x * a.scale : 0.0f;
+// A dropped element counts as zero whatever x holds there, NaN and infinities included.  Product and
+// sum are one operation with one rounding, in both kernels.
+__device__ __forceinline__ float drop(const DropoutArgs& a, u32 word, float x, float residual) {
+  return fmaf(word >= a.threshold && !a.drop_all ? x : 0.0f, a.scale, residual);
 }
 
 constexpr int kDropUnroll = 4;  // 16-byte vectors per thread
@@ -130,10 +131,13 @@ __global__ void __launch_bounds__(kBlock) dropout_dense_kernel(const __grid_cons
       u32 w[4];
       philox_planned((u32)v * (u32)(V / 4) + (u32)b, plan, w);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float d = w[j] >= a.threshold ? f[4 * b + j] * a.scale : 0.0f;
-        if constexpr (RES) y[4 * b + j] += d;
-        else y[4 * b + j] = d;
+      for (int j = 0; j < 4; j += 2) {
+        const int i = 4 * b + j;
+        const Two kept(w[j] >= a.threshold ? f[i] : 0.0f, w[j + 1] >= a.threshold ? f[i + 1] : 0.0f), scale(a.scale, a.scale);
+        Two r;
+        if constexpr (RES) r = fma(kept, scale, Two(y[i], y[i + 1]));
+        else r = mul(kept, scale);
+        r.get(y[i], y[i + 1]);
       }
     }
     st_v4(out + v * V, pack(y, static_cast<const T*>(nullptr)));
@@ -144,8 +148,9 @@ __global__ void __launch_bounds__(kBlock) dropout_dense_kernel(const __grid_cons
     u32 w[4];
     philox_planned((u32)(i >> 2), plan, w);
     const u32 word = i & 2 ? (i & 1 ? w[3] : w[2]) : (i & 1 ? w[1] : w[0]);
-    float y = word >= a.threshold ? to_f32(x[i]) * a.scale : 0.0f;
-    if constexpr (RES) y += to_f32(res[i]);
+    const float kept = word >= a.threshold ? to_f32(x[i]) : 0.0f;
+    float y = kept * a.scale;
+    if constexpr (RES) y = fmaf(kept, a.scale, to_f32(res[i]));
     out[i] = from_f32<T>(y);
   }
 }
@@ -172,9 +177,8 @@ __global__ void __launch_bounds__(kBlock) dropout_strided_kernel(const __grid_co
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (4 * blk + j >= n) break;
-      float y = drop(a, w[j], x[j]);
-      if constexpr (RES) y += r[j];
-      static_cast<T*>(a.out)[off[j][0]] = from_f32<T>(y);
+      // without a residual -0: a product of -0 keeps its sign
+      static_cast<T*>(a.out)[off[j][0]] = from_f32<T>(drop(a, w[j], x[j], RES ? r[j] : -0.0f));
     }
   }
 }

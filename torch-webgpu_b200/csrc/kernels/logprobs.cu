@@ -244,22 +244,30 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
   // Every thread copies its own vectors to its own places in shared memory and reads them back, so a
   // stage needs no barrier, and what is on its way takes no registers.
   const int each = nt * kLpUnroll, n = v1 - v0;
-  auto fetch = [&](int q) {
+  // (FULL: a stage of which every thread has all its vectors, which is every one but a row's last.)
+  const int full = n / each;
+  auto fetch_as = [&](int q, bool whole) {
     uint4* to = ring + (q & (kLpStages - 1)) * each + tid;
     const int v = v0 + q * each + tid;
+    const T* from = row + rs.head + (i64)v * V;
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k)
-      if (v + k * nt < v1) copy_async(to + k * nt, row + rs.head + (i64)(v + k * nt) * V);
+      if (whole || v + k * nt < v1) copy_async(to + k * nt, from + (i64)k * nt * V);
+  };
+  auto fetch = [&](int q) {
+    if (q < full) fetch_as(q, true);
+    else fetch_as(q, false);
     copy_async_commit();
   };
-  auto take = [&](int q, float (&f)[kLpUnroll * V]) {
+  auto take_as = [&](int q, float (&f)[kLpUnroll * V], bool whole) {
     const uint4* from = ring + (q & (kLpStages - 1)) * each + tid;
     const int v = v0 + q * each + tid;
     float largest = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k) {
-      uint4 raw = minus_inf<T>();
-      if (v + k * nt < v1) raw = from[k * nt];
+      uint4 raw;
+      if (whole || v + k * nt < v1) raw = from[k * nt];
+      else raw = minus_inf<T>();
       float g[V];
       unpack(raw, g, static_cast<const T*>(nullptr));
 #pragma unroll
@@ -269,6 +277,9 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
       }
     }
     return largest;
+  };
+  auto take = [&](int q, float (&f)[kLpUnroll * V]) {
+    return q < full ? take_as(q, f, true) : take_as(q, f, false);
   };
 #pragma unroll
   for (int q = 0; q < kLpStages; ++q) fetch(q);

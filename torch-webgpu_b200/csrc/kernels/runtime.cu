@@ -931,13 +931,6 @@ extern "C" int twg_host_alloc_pinned(void** ptr, size_t nbytes) {
   return TWG_OK;
 }
 
-extern "C" int twg_host_is_pinned(const void* ptr, int* pinned) {
-  TWG_REQUIRE(pinned != nullptr, "twg_host_is_pinned: null argument");
-  int n = 0;
-  *pinned = ptr && device_count_cached(&n) == TWG_OK && n > 0 && is_pinned(ptr) ? 1 : 0;
-  return TWG_OK;
-}
-
 extern "C" int twg_host_free_pinned(void* ptr) {
   if (ptr) TWG_CUDA(cudaFreeHost(ptr));
   return TWG_OK;

@@ -139,7 +139,6 @@ SIGNATURES = {
     "twg_memset": (c_int, [c_void_p, c_int, c_size_t, c_void_p]),
     "twg_host_alloc_pinned": (c_int, [POINTER(c_void_p), c_size_t]),
     "twg_host_free_pinned": (c_int, [c_void_p]),
-    "twg_host_is_pinned": (c_int, [c_void_p, POINTER(c_int)]),
     "twg_copy_strided": (c_int, [POINTER(IterDesc), c_int, c_void_p, c_void_p, c_void_p]),
     "twg_fill": (c_int, [POINTER(IterDesc), c_int, ctypes.c_uint64, c_void_p, c_void_p]),
     "twg_unary_f32": (c_int, [c_int, POINTER(IterDesc), c_void_p, c_void_p, c_void_p]),

@@ -401,6 +401,10 @@ def test_dropout_state_and_second_gradient():
     state = torch.tensor([-5, 40]).to("webgpu")
     y = ops.dropout_state(xd, 0.25, state, 2)
     check_dropout(y, x, 0.25, -5, 42, None, "state")
+    for dtype in DTYPES:                                    # the dense kernel's own plan, and the strided one
+        big, res = rand(9, 1000, dtype=dtype), rand(9, 1000, dtype=dtype, seed=5)
+        check_dropout(ops.dropout_state(big.to("webgpu"), 0.25, state, -1, residual=res.to("webgpu")), big, 0.25, -5, 39, res, "dense state")
+        check_dropout(ops.dropout_state(big.to("webgpu").t(), 0.25, state, -41), big.t(), 0.25, -5, -1, None, "strided state")
     g = rand(3, 50, seed=1).to("webgpu").requires_grad_()
     (dx,) = torch.autograd.grad(y, xd, g, create_graph=True)
     check_dropout(dx, g.cpu().detach(), 0.25, -5, 42, None, "gradient")

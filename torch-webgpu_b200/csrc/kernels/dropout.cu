@@ -45,9 +45,10 @@ __device__ __forceinline__ void philox_block(u64 block, u64 seed, u64 offset, u3
 struct PhiloxPlan {
   u32 x[10][2];  // what words 0 and 2 of each round are combined with besides the products' halves
 };
-static PhiloxPlan make_plan(u64 seed, u64 offset) {
+__host__ __device__ __forceinline__ PhiloxPlan make_plan(u64 seed, u64 offset) {
   PhiloxPlan p;
   u32 k0 = (u32)seed, k1 = (u32)(seed >> 32);
+#pragma unroll
   for (int i = 0; i < 10; ++i) {
     p.x[i][0] = k0;
     p.x[i][1] = k1;
@@ -100,10 +101,10 @@ __device__ __forceinline__ float drop(const DropoutArgs& a, u32 word, float x, f
 
 constexpr int kDropUnroll = 4;  // 16-byte vectors per thread
 
-// Dense operands of fewer than 2^34 elements, the seed and offset from the host and p below 1: `vecs`
-// whole 16-byte vectors; the last CTA also takes the tail of n.
-template <class T, bool RES>
-__global__ void __launch_bounds__(kBlock) dropout_dense_kernel(const __grid_constant__ DropoutArgs a, const __grid_constant__ PhiloxPlan plan,
+// Dense operands of fewer than 2^34 elements and p below 1: `vecs` whole 16-byte vectors; the last CTA
+// also takes the tail of n.  STATE: seed and offset are on the device, every thread works its plan out.
+template <class T, bool RES, bool STATE>
+__global__ void __launch_bounds__(kBlock) dropout_dense_kernel(const __grid_constant__ DropoutArgs a, const __grid_constant__ PhiloxPlan host_plan,
                                                                 i64 vecs, i64 n) {
   constexpr int V = kVecOf<T>;
   const T* x = static_cast<const T*>(a.x);
@@ -119,6 +120,13 @@ __global__ void __launch_bounds__(kBlock) dropout_dense_kernel(const __grid_cons
       if constexpr (RES) rr[k] = ld_v4(res + v * V);
     }
   }
+  PhiloxPlan own;
+  if constexpr (STATE) {
+    u64 seed, offset;
+    load_state(a, &seed, &offset);
+    own = make_plan(seed, offset);
+  }
+  const PhiloxPlan& plan = STATE ? own : host_plan;
 #pragma unroll
   for (int k = 0; k < kDropUnroll; ++k) {
     const i64 v = base + k * kBlock;
@@ -155,7 +163,7 @@ __global__ void __launch_bounds__(kBlock) dropout_dense_kernel(const __grid_cons
   }
 }
 
-// Any strides, a seed on the device, p = 1: a thread takes the four elements of one block, one after the
+// Any strides, p = 1, 2^34 elements and more: a thread takes the four elements of one block, one after the
 // other along dimension 0.
 template <class T, bool RES, class IDX>
 __global__ void __launch_bounds__(kBlock) dropout_strided_kernel(const __grid_constant__ DropoutArgs a, const __grid_constant__ StridedDesc<3, IDX> d, i64 n) {
@@ -192,8 +200,10 @@ static int launch_dropout(const DropoutArgs& a, const TwgIterDesc& d, cudaStream
   if (dense) {
     const i64 vecs = d.numel / V, per = kBlock * kDropUnroll;
     const i64 grid = std::max<i64>(1, (vecs + per - 1) / per);
-    if (d.numel < (i64(1) << 34) && !a.state && !a.drop_all) {
-      dropout_dense_kernel<T, RES><<<(unsigned)grid, kBlock, 0, s>>>(a, make_plan(a.seed, a.offset), vecs, d.numel);
+    if (d.numel < (i64(1) << 34) && !a.drop_all) {
+      const PhiloxPlan plan = make_plan(a.seed, a.offset);
+      if (a.state) dropout_dense_kernel<T, RES, true><<<(unsigned)grid, kBlock, 0, s>>>(a, plan, vecs, d.numel);
+      else dropout_dense_kernel<T, RES, false><<<(unsigned)grid, kBlock, 0, s>>>(a, plan, vecs, d.numel);
       TWG_CHECK_LAUNCH();
       g_last_path = kPathDense;
       return TWG_OK;

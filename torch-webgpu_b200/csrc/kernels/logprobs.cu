@@ -204,6 +204,7 @@ __device__ __forceinline__ void rank_keys(const u64* keys, int n, int top, u64* 
   for (int i = threadIdx.x; i < n; i += (int)blockDim.x) {
     const u64 k = keys[i];
     int r = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) r += keys[j] > k;
     if (k != 0 && r < top) best[r] = k;
   }
@@ -232,6 +233,18 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
   const bool extra = part == 0 && tid < rs.head + rs.tail;
   const int i_extra = tid < rs.head ? tid : a.vocab - rs.tail + tid - rs.head;
   float fx[1] = {extra ? to_f32(row[i_extra]) : -INFINITY};
+
+  // the given tokens' logits, asked for before anything else is waited for
+  auto token = [&](int j) {
+    const i64 at = r * a.ts0 + j * a.ts1;
+    return a.tok64 ? static_cast<const i64*>(a.tokens)[at] : (i64) static_cast<const int*>(a.tokens)[at];
+  };
+  i64 tok = -1;
+  float x_tok = 0.0f;
+  if (part == 0 && tid < a.m) {
+    tok = token(tid);
+    if (tok >= 0 && tok < a.vocab) x_tok = to_f32(row[tok]);
+  }
 
   SoftPair mine;
   float limit = INFINITY;  // only elements that reach it can be among the alternatives
@@ -372,11 +385,13 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
     a.entropy[r] = none ? 0.0f : ln_s - kLn2 * (soft.t / soft.s);
   }
   for (int j = tid; j < a.m; j += nt) {
-    const i64 at = r * a.ts0 + j * a.ts1;
-    const i64 tok = a.tok64 ? static_cast<const i64*>(a.tokens)[at] : (i64) static_cast<const int*>(a.tokens)[at];
+    if (j != tid) {
+      tok = token(j);
+      if (tok >= 0 && tok < a.vocab) x_tok = to_f32(row[tok]);
+    }
     float lp = 0.0f;                              // a negative token is padding
     if (tok >= a.vocab) lp = as_f(0x7fffffffu);   // one that does not exist has no probability to report
-    else if (tok >= 0) lp = log_prob(to_f32(row[tok]));
+    else if (tok >= 0) lp = log_prob(x_tok);
     a.logp[r * a.m + j] = lp;
   }
   if constexpr (TOP) {

@@ -821,6 +821,97 @@ def test_a_training_step_of_all_of_them():
         assert err <= 4 * (R.LN_S + 16 * (R.NORM + R.TURN) + 3 * R.RNORM + 100 * R.U), float(err)
 
 
+def test_nothing_is_written_behind_the_outputs(abi):
+    """Guard words behind every block of the allocator, odd sizes of everything."""
+    L = abi.lib()
+    abi.check(L.twg_set_guard_words(1))
+    keep = []
+    try:
+        for dtype in DTYPES:
+            for d, r in ((64, 64), (72, 72), (100, 50), (7, 4)):
+                q, k = rand(1, 13, 5, d, dtype=dtype).to("webgpu").requires_grad_(), rand(1, 13, 1, d, dtype=dtype).to("webgpu").requires_grad_()
+                w = torch.ones(d, dtype=dtype).to("webgpu").requires_grad_()
+                pos, f = torch.arange(13).to("webgpu"), freqs(r).to("webgpu")
+                out = ops.qk_norm_rotary(q, k, w, w.detach().clone().requires_grad_(), pos, f)
+                keep += [q, k, w, pos, f, *out, *ops.rotary_qk(q, k, pos, f)]
+                keep += torch.autograd.grad(out, (q, k, w), [torch.empty_like(o).fill_(1) for o in out])
+            for n in (1, 7, 1001):
+                x = rand(n, dtype=dtype).to("webgpu")
+                keep += [x, ops.dropout(x, 0.3, 1), ops.dropout(x, 0.3, 1, residual=x)]
+            for rows, vocab, top in ((1, 5, 5), (3, 1003, 7), (2, 40001, 20)):
+                x = rand(rows, vocab, dtype=dtype).to("webgpu").requires_grad_()
+                out = ops.token_logprobs(x, torch.zeros(rows, 3, dtype=torch.long).to("webgpu"), top=top)
+                keep += [x, *out, torch.autograd.grad(out[0], x, torch.empty_like(out[0]).fill_(1))[0]]
+        bad, first = ctypes.c_int64(-1), ctypes.c_void_p()
+        abi.check(L.twg_check_guard_words(0, ctypes.byref(bad), ctypes.byref(first)))
+        assert bad.value == 0, f"{bad.value} blocks were written behind their end, the first at {first.value:#x}"
+    finally:
+        abi.check(L.twg_set_guard_words(0))
+
+
+def test_offsets_beyond_32_bits(abi):
+    """C ABI: strides that put the second token, row or slice more than 2^31 elements behind the first."""
+    L, far, d = abi.lib(), 2 ** 31 + 64, 128
+    buf = torch.zeros(far + 4096, dtype=torch.bfloat16, device="cuda")
+    x = rand(2, 2, d, dtype=torch.bfloat16)
+    buf[:2 * d], buf[far:far + 2 * d] = x[0].reshape(-1).cuda(), x[1].reshape(-1).cuda()
+    st = torch.cuda.current_stream().cuda_stream
+    pos, f = torch.arange(2, device="cuda") + 5, freqs(d).cuda()
+    wide, dense = (0, far, d, 1), (0, 2 * d, d, 1)
+    out = torch.empty(1, 2, 2, d, dtype=torch.bfloat16, device="cuda")
+    ang = R.angles(pos.cpu()[None, None], f.cpu(), [0] * (d // 2), (1, 2))
+    desc = abi.rotary_desc("bf16", (1, 2), (2, 0), d, in_strides=(wide, wide), out_strides=(dense, dense), grad_strides=(wide, wide),
+                           position_strides=(0, 0, 1), eps=1e-5)
+    abi.check(L.twg_rotary(ctypes.byref(desc), buf.data_ptr(), None, pos.data_ptr(), f.data_ptr(), out.data_ptr(), None, st))
+    R.assert_within(out, R.turn(x[None].double(), ang, False), R.TURN * R.pair_size(x[None].double(), d, False), "far token")
+    ws = torch.empty(L.twg_qk_norm_rotary_workspace_bytes(ctypes.byref(desc)), dtype=torch.uint8, device="cuda")
+    abi.check(L.twg_qk_norm_rotary_backward(ctypes.byref(desc), buf.data_ptr(), None, None, None, pos.data_ptr(), f.data_ptr(), buf.data_ptr(), None,
+                                            out.data_ptr(), None, None, None, ws.data_ptr(), ws.numel(), st))
+    _, _, dx, dxb, _, _ = norm_reference(x[None], None, x[None], ang, d, False, float(np.float32(1e-5)))
+    R.assert_within(out, dx, dxb, "far gradient")
+
+    rows = x.reshape(2, 2 * d)
+    tokens, numbers = torch.tensor([3, 200], device="cuda"), torch.empty(3, 2, device="cuda")
+    top_logp, ids = torch.empty(2, 4, device="cuda"), torch.empty(2, 4, dtype=torch.long, device="cuda")
+    ld = abi.logprobs_desc("bf16", 2, 2 * d, row_stride=far, token_strides=(1, 1), top=4)
+    abi.check(L.twg_token_logprobs(ctypes.byref(ld), buf.data_ptr(), tokens.data_ptr(), numbers[0].data_ptr(), numbers[1].data_ptr(),
+                                   numbers[2].data_ptr(), top_logp.data_ptr(), ids.data_ptr(), st))
+    check_logprobs([numbers[0][:, None], numbers[1], numbers[2], top_logp, ids], rows, tokens.cpu()[:, None], 1.0, 4)
+
+    it = abi.make_desc((2, 2 * d), [((2, 2 * d), (2 * d, 1)), ((2, 2 * d), (far, 1))])
+    abi.check(L.twg_dropout(ctypes.byref(it), abi.DTYPES["bf16"], buf.data_ptr(), None, out.data_ptr(), 0.5, 3, 4, None, st))
+    assert abi.last_path() == "strided64"
+    check_dropout(out.view(2, 2 * d), rows, 0.5, 3, 4, None, "far rows")
+    grad = torch.zeros_like(buf)
+    abi.check(L.twg_token_logprobs_backward(ctypes.byref(ld), buf.data_ptr(), tokens.data_ptr(), None, numbers[2].data_ptr(), numbers[1].data_ptr(),
+                                            None, None, grad.data_ptr(), far, st))
+    got = torch.stack([grad[:2 * d], grad[far:far + 2 * d]]).cpu()
+    zero = torch.zeros(2)
+    check_logprobs_grad(got, rows, tokens.cpu()[:, None], 1.0, numbers[1].cpu()[:, None], zero, zero)
+    assert not bool(grad[2 * d:far].any())
+
+
+def test_dropout_of_more_than_2_to_34_elements(abi):
+    """Blocks whose number needs more than 32 bits, in place."""
+    n = 2 ** 34 + 1027
+    if torch.cuda.mem_get_info()[0] < 2 * n + (8 << 30):
+        pytest.skip("needs 42 GB of free memory")
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    d = abi.IterDesc()
+    abi.check(abi.lib().twg_iter_contiguous(ctypes.byref(d), 2, n))
+    abi.check(abi.lib().twg_dropout(ctypes.byref(d), abi.DTYPES["bf16"], x.data_ptr(), None, x.data_ptr(), 0.5, 77, 5, None,
+                                    torch.cuda.current_stream().cuda_stream))
+    for lo in (0, 2 ** 33 - 512, 2 ** 34 - 1024, n - 1027):
+        lo, hi = lo // 4 * 4, min(n, lo // 4 * 4 + 1028)
+        block = np.arange(lo // 4, (hi + 3) // 4, dtype=np.uint64)
+        same = np.ones_like(block)
+        words = R.philox([block & np.uint64(0xFFFFFFFF), block >> np.uint64(32), same * np.uint64(5), same * np.uint64(0)], [77, 0]).T.reshape(-1)
+        keep = torch.from_numpy(words >= np.uint64(2 ** 31))[:hi - lo]
+        assert torch.equal(x[lo:hi].cpu().float(), torch.where(keep, 2.0, 0.0)), lo
+    del x
+    torch.cuda.empty_cache()
+
+
 def test_second_device_is_honoured(abi):
     if torch.cuda.device_count() < 2:
         pytest.skip("needs two GPUs")

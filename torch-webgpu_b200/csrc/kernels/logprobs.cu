@@ -15,6 +15,12 @@
 // everything else has to stay at a few instructions an element.  A row belongs to a cluster of 1
 // to 8 CTAs which combine their numbers through distributed shared memory: few long rows still
 // fill the GPU, nothing passes through a workspace and there is one launch.
+//
+// 4096 rows of 131072 bfloat16 logits: forward 185 us (5.8 TB/s), 221 us under a load of seconds (power
+// limit), gradient 319 us (6.7 TB/s, the copy bandwidth).  2047 rows of 50257 float32 logits with five
+// alternatives 70 us, 79 us under that load.  Measured and dropped: loads held in registers (207 us, and
+// 247 with 512 threads a row), CTAs that stay for several rows (226 us), stages of four vectors (181 us,
+// but 73 us for the float32 rows).
 #include <cooperative_groups.h>
 
 #include <cfloat>

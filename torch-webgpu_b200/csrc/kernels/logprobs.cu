@@ -216,8 +216,8 @@ __device__ __forceinline__ void rank_keys(const u64* keys, int n, int top, u64* 
   }
 }
 
-template <class T, bool TOP>
-__global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+template <class T, bool TOP, int NT>
+__global__ void __launch_bounds__(NT, kLpCtas * (kLpMaxThreads / NT)) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
   constexpr int V = kVecOf<T>;
   __shared__ LpShared sh;
   extern __shared__ uint4 ring[];  // [kLpStages][kLpUnroll][threads]
@@ -228,7 +228,8 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
   const RowSplit<T> rs(row, a.vocab);
   const int per = (rs.nvec + parts - 1) / parts;
   const int v0 = min(part * per, rs.nvec), v1 = min(v0 + per, rs.nvec);
-  const int tid = threadIdx.x, nt = blockDim.x;
+  constexpr int nt = NT;
+  const int tid = threadIdx.x;
   const float c = a.scale * kLog2e;
   if constexpr (TOP) {
     if (tid == 0) sh.count = 0;
@@ -262,30 +263,30 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
   };
   // Every thread copies its own vectors to its own places in shared memory and reads them back, so a
   // stage needs no barrier, and what is on its way takes no registers.
-  const int each = nt * kLpUnroll, n = v1 - v0;
-  // (FULL: a stage of which every thread has all its vectors, which is every one but a row's last.)
-  const int full = n / each;
-  auto fetch_as = [&](int q, bool whole) {
-    uint4* to = ring + (q & (kLpStages - 1)) * each + tid;
-    const int v = v0 + q * each + tid;
-    const T* from = row + rs.head + (i64)v * V;
-#pragma unroll
-    for (int k = 0; k < kLpUnroll; ++k)
-      if (whole || v + k * nt < v1) copy_async(to + k * nt, from + (i64)k * nt * V);
-  };
+  // (`whole`: a stage of which every thread has all its vectors, which is every one but a row's last.)
+  constexpr int each = nt * kLpUnroll;
+  const int n = v1 - v0, full = n / each;
+  const T* from = row + rs.head + (i64)(v0 + tid) * V;  // of the next stage to be fetched
   auto fetch = [&](int q) {
-    if (q < full) fetch_as(q, true);
-    else fetch_as(q, false);
+    uint4* to = ring + (q & (kLpStages - 1)) * each + tid;
+    if (q < full) {
+#pragma unroll
+      for (int k = 0; k < kLpUnroll; ++k) copy_async(to + k * nt, from + k * nt * V);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kLpUnroll; ++k)
+        if (q * each + k * nt + tid < n) copy_async(to + k * nt, from + k * nt * V);
+    }
+    from += each * V;
     copy_async_commit();
   };
-  auto take_as = [&](int q, float (&f)[kLpUnroll * V], bool whole) {
-    const uint4* from = ring + (q & (kLpStages - 1)) * each + tid;
-    const int v = v0 + q * each + tid;
+  auto take = [&](int q, float (&f)[kLpUnroll * V], bool whole) {
+    const uint4* at = ring + (q & (kLpStages - 1)) * each + tid;
     float largest = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kLpUnroll; ++k) {
       uint4 raw;
-      if (whole || v + k * nt < v1) raw = from[k * nt];
+      if (whole || q * each + k * nt + tid < n) raw = at[k * nt];
       else raw = minus_inf<T>();
       float g[V];
       unpack(raw, g, static_cast<const T*>(nullptr));
@@ -297,9 +298,6 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
     }
     return largest;
   };
-  auto take = [&](int q, float (&f)[kLpUnroll * V]) {
-    return q < full ? take_as(q, f, true) : take_as(q, f, false);
-  };
 #pragma unroll
   for (int q = 0; q < kLpStages; ++q) fetch(q);
   float f[kLpUnroll * V];
@@ -309,7 +307,7 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
     copy_async_wait<0>();
     float largest = fx[0];
 #pragma unroll 1
-    for (int q = 0; q < kLpStages; ++q) largest = fmaxf(largest, take(q, f));
+    for (int q = 0; q < kLpStages; ++q) largest = fmaxf(largest, take(q, f, false));
     u32 own = extra || tid < n ? order_of(largest) >> 16 : 0;
     if (own > 0xff80u) own = 0xff80u;  // a NaN: the slow way will see it
     u32 prefix = 0;
@@ -320,25 +318,27 @@ __global__ void __launch_bounds__(kLpMaxThreads, kLpCtas) logprobs_kernel(const 
     limit = prefix <= 0x7fu ? -INFINITY : value_of(prefix << 16);
     if (extra) push(fx[0], i_extra);
   }
-#pragma unroll 1
-  for (int q = 0; q * each < n; ++q) {
+  auto work = [&](int q, bool whole) {
     copy_async_wait<kLpStages - 1>();
-    const float largest = take(q, f);
+    const float largest = take(q, f, whole);
     fetch(q + kLpStages);
     mine.add_all(f, largest, c);
     if constexpr (TOP) {
       if (largest >= limit) {
 #pragma unroll
         for (int k = 0; k < kLpUnroll; ++k) {
-          const int v = v0 + q * each + k * nt + tid;
-          if (v < v1) {
+          const int v = q * each + k * nt + tid;
+          if (v < n) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) push(f[k * V + j], rs.head + v * V + j);
+            for (int j = 0; j < V; ++j) push(f[k * V + j], rs.head + (v0 + v) * V + j);
           }
         }
       }
     }
-  }
+  };
+#pragma unroll 1
+  for (int q = 0; q < full; ++q) work(q, true);
+  if (full * each < n) work(full, false);
   copy_async_wait<0>();
   Soft soft = mine.sum();
   soft.add(fx, fx[0], c);
@@ -582,10 +582,9 @@ static int launch_logprobs(const LogprobArgs& a, int64_t rows, cudaStream_t s) {
   // CTAs per row: as many as keep two on every SM, while each still has a round of its threads' loads
   int parts = 1;
   while (parts < kLpMaxCluster && rows * parts * 2 <= 2 * sm_count() && nvec / (parts * 2) >= 256) parts *= 2;
-  // threads: a warp's worth of vectors each where the row is short
+  // half the threads where a row has no vector for every one of them
   const int each = (nvec + parts - 1) / parts;
-  int threads = 128;
-  while (threads < kLpMaxThreads && threads * 2 <= each) threads *= 2;
+  const int threads = each < kLpMaxThreads ? kLpMaxThreads / 2 : kLpMaxThreads;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * parts));
   cfg.blockDim = dim3((unsigned)threads);
@@ -596,8 +595,9 @@ static int launch_logprobs(const LogprobArgs& a, int64_t rows, cudaStream_t s) {
   attr[0].val.clusterDim = {(unsigned)parts, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (a.top) TWG_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<T, true>, a));
-  else TWG_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<T, false>, a));
+  const bool small = threads < kLpMaxThreads;
+  if (a.top) TWG_CUDA(cudaLaunchKernelEx(&cfg, small ? logprobs_kernel<T, true, kLpMaxThreads / 2> : logprobs_kernel<T, true, kLpMaxThreads>, a));
+  else TWG_CUDA(cudaLaunchKernelEx(&cfg, small ? logprobs_kernel<T, false, kLpMaxThreads / 2> : logprobs_kernel<T, false, kLpMaxThreads>, a));
   TWG_CHECK_LAUNCH();
   return TWG_OK;
 }

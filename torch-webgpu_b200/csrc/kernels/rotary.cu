@@ -37,7 +37,7 @@ struct RotaryArgs {
   i64 ps[3];  // axis, batch, seq
   const void* freq;
   u32 seq, tokens;
-  int D, R, slots, lanes;  // lanes: lanes of a row's group (a power of two)
+  int D, R, slots, lanes;  // lanes: of a row's group (a power of two where a sum goes over it)
   int tile, head_span, parts;  // forward: tokens and heads per warp, warps per token
   int step[2];             // backward: heads of q and of k that one round of a warp's lane groups takes (a power of two)
   int ctas[2];             // CTAs that work on q and on k (backward)
@@ -327,13 +327,13 @@ __global__ void __launch_bounds__(kRotThreads, V == 8 ? 5 : V > 1 ? 4 : 1) rotar
   }
   __syncwarp();
 
-  const int lanes = LANES ? LANES : a.lanes, groups = 32 / lanes, p0 = lane & (lanes - 1);
+  const int lanes = LANES ? LANES : a.lanes, groups = 32 / lanes, group = lane / lanes, p0 = lane - group * lanes;
   int e0[NS], e1[NS];
   bool has[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
     slot_elems(a, p0 + 32 * i, V, &e0[i], &e1[i]);
-    has[i] = p0 + 32 * i < a.slots;
+    has[i] = p0 + 32 * i < a.slots && group < groups;
   }
   Row<T, V, NS> x;
   x.clear();
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kRotThreads, V == 8 ? 5 : V > 1 ? 4 : 1) rotar
     x.load(static_cast<const T*>(a.x[z]) + (on ? offs[at.t][z] : 0) + (i64)(h - (z ? a.heads[0] : 0)) * a.xs[z][2], a.xs[z][3], e0, e1, has,
            a.D, on);
   };
-  Place at(lane / lanes, span);
+  Place at(group, span);
   fetch(at);
   for (int t = 0; t < ntok; ++t) {
     i64 b, s;
@@ -431,9 +431,9 @@ __global__ void __launch_bounds__(kRotThreads, V == 8 ? 5 : V > 1 ? 4 : 1) rotar
 // Cosines and sines of the gradient's tokens: [tokens][2][slots V], quads of a slot as in shared memory.
 // A thread keeps its frequency, as a 64-bit fraction of a turn: positions are whole numbers, so the
 // product modulo 2^64 is the angle without its whole turns.
-constexpr int kRotTableTokens = 16;  // tokens of a thread
+constexpr int kRotTableTokens = 16;  // tokens of a thread, at most
 template <int V>
-__global__ void __launch_bounds__(kRotThreads) rotary_table_kernel(const __grid_constant__ RotaryArgs a, float* table) {
+__global__ void __launch_bounds__(kRotThreads) rotary_table_kernel(const __grid_constant__ RotaryArgs a, float* table, int each) {
   const int row = a.slots * V, f = blockIdx.y * blockDim.x + threadIdx.x;
   if (f >= row) return;
   const bool turned = f < (a.R >> 1);
@@ -446,8 +446,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_table_kernel(const __grid_
     part = __double2ull_rn(turns * 18446744073709551616.0);
   }
   const i64 axis = turned ? (i64)a.axis_of[f] * a.ps[0] : 0;
-  const i64 first = ((i64)blockIdx.x * blockDim.y + threadIdx.y) * kRotTableTokens;
-  for (i64 tok = first; tok < min(first + kRotTableTokens, (i64)a.tokens); ++tok) {
+  const i64 first = ((i64)blockIdx.x * blockDim.y + threadIdx.y) * each;
+  for (i64 tok = first; tok < min(first + each, (i64)a.tokens); ++tok) {
     float c = 1.0f, s = 0.0f;
     if (turned) {
       i64 b, q;
@@ -801,6 +801,8 @@ static void by_lanes(int lanes, Fn&& fn) {
 template <class T, int V, int NS, bool ADJ>
 static int launch_forward(RotaryArgs& a, bool norm, cudaStream_t s) {
   set_slots(&a, V);
+  // without a sum over the head a group may have as many lanes as slots: three rows of ten slots to a warp
+  if (!norm && V > 1) a.lanes = a.slots;
   const int H = a.heads[0] + a.heads[1], row = a.slots * V;
   const int groups = 32 / a.lanes;
   // rows per warp: what leaves 40 warps to an SM, between one round of the lane groups and kRotRounds
@@ -909,19 +911,18 @@ static int launch_grad(RotaryArgs& a, float* table, cudaStream_t s) {
   }
   int wide = 32;  // threads along the frequencies, the rest of a CTA along the tokens
   while (wide < row && wide < kRotThreads) wide *= 2;
-  const int high = kRotThreads / wide, per = high * kRotTableTokens;
-  rotary_table_kernel<V><<<dim3((a.tokens + per - 1) / per, (row + wide - 1) / wide), dim3(wide, high), 0, s>>>(a, table);
+  // tokens of a thread: what leaves eight CTAs to an SM (they come one after the other)
+  const int high = kRotThreads / wide;
+  const int each = (int)std::min<int64_t>(std::max<int64_t>((int64_t)a.tokens * wide / ((int64_t)sm_count() * 8 * kRotThreads), 1), kRotTableTokens);
+  const int per = high * each;
+  rotary_table_kernel<V><<<dim3((a.tokens + per - 1) / per, (row + wide - 1) / wide), dim3(wide, high), 0, s>>>(a, table, each);
   TWG_CHECK_LAUNCH();
   a.table = table;
   const size_t smem = sizeof(float) * (size_t)row * 2 + std::max(sizeof(float) * (size_t)row * 2 * kRotWarps,
                                                                  V > 1 ? sizeof(T) * V * 4 * kRotStages * kRotThreads : (size_t)0);
-  cudaError_t err = cudaSuccess;
   by_lanes<V == kVecOf<T>>(a.lanes, [&](auto lanes) {
-    const auto kernel = rotary_grad_kernel<T, V, NS, ADJ, decltype(lanes)::value>;
-    if (smem > 48 * 1024) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (err == cudaSuccess) kernel<<<a.ctas[0] + a.ctas[1], kRotThreads, smem, s>>>(a);
+    rotary_grad_kernel<T, V, NS, ADJ, decltype(lanes)::value><<<a.ctas[0] + a.ctas[1], kRotThreads, smem, s>>>(a);
   });
-  TWG_CUDA(err);
   TWG_CHECK_LAUNCH();
   g_last_path = V == 1 ? kPathStrided64 : kPathDense;
   return TWG_OK;

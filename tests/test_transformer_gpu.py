@@ -441,6 +441,22 @@ def test_torch_dropout_module():
     check_dropout(torch.nn.functional.dropout(xd, 0.5), x, 0.5, -1, 0, None, "negative seed")
 
 
+def test_checkpointed_dropout_draws_the_same_mask_again():
+    from torch.utils.checkpoint import checkpoint
+    drop = torch.nn.Dropout(0.5)
+    x = rand(40, 50).to("webgpu").requires_grad_()
+    torch.webgpu.manual_seed(5)
+    drop(x)                                               # the generator does not stand at its start
+    y = checkpoint(lambda t: drop(t) * 2.0, x, use_reentrant=False)
+    after = torch.webgpu.get_rng_state()
+    (dx,) = torch.autograd.grad(y, x, torch.ones(40, 50).to("webgpu"))
+    assert torch.equal(dx.cpu() != 0, R.keep_mask((40, 50), 0.5, 5, 1)) and torch.equal(y.detach().cpu() != 0, dx.cpu() != 0)
+    assert torch.equal(torch.webgpu.get_rng_state(), after)
+    with torch.random.fork_rng(devices=[0], device_type="webgpu"):
+        drop(x)
+    assert torch.equal(torch.webgpu.get_rng_state(), after)
+
+
 # ------------------------------------------------------------------------------------------
 # token log probabilities
 # ------------------------------------------------------------------------------------------
@@ -608,6 +624,11 @@ def test_token_logprobs_layouts(dtype):
     out = ops.token_logprobs(on.view(13, 1, 1007).requires_grad_(), tok[:, :1].to("webgpu"), scale=1.25)
     assert out[0].shape == (13, 1) and out[1].shape == (13, 1)
     assert ops.token_logprobs(torch.empty(0, 50, device="webgpu"), torch.empty(0, dtype=torch.long, device="webgpu"))[0].shape == (0,)
+    x = on.detach().requires_grad_()
+    none = ops.token_logprobs(x, torch.empty(13, 0, dtype=torch.long, device="webgpu"), top=1)
+    assert none[0].shape == (13, 0)
+    (dx,) = torch.autograd.grad(none[2], x, torch.ones(13).to("webgpu"))
+    check_logprobs_grad(dx, base, tok[:, :0], 1.0, torch.zeros(13, 0), torch.zeros(13), torch.ones(13), "no tokens")
     single = ops.token_logprobs(on[3], tok[3, 0].to("webgpu"), top=2)
     assert single[0].shape == () and single[3].shape == (2,)
     with pytest.raises(RuntimeError, match="once only"):

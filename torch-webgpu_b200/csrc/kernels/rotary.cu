@@ -299,12 +299,13 @@ struct Place {
 // Forward: every warp works by itself on `tile` tokens and `head_span` of their q and k heads, about
 // kRotRounds rows to a lane group.  It issues the loads of its first rows, forms the tables while
 // they travel, and from then on always has the next rows on their way.  16384 tokens of 32 + 8 heads
-// of 128 in bfloat16 take 60.8 us (5.5 TB/s, 84 % of the copy bandwidth).  Measured and dropped: tables
+// of 128 in bfloat16 take 60.9 us (5.5 TB/s, 84 % of the copy bandwidth; 61.7 with five CTAs an SM, whose
+// 48 registers spill, 64.9 with three).  Measured and dropped: tables
 // of a CTA behind a barrier 63.9 us; no loop, one or two rows to a lane group 76 and 61 us (82 us where
 // the norm's weights add to what a CTA does first, 59.7 us here); the cosines of a token in registers
 // and rows two at a time 66 to 70 us; angles from 64-bit fractions of a turn instead of float64 65 us.
 template <class T, int V, int NS, bool NORM, bool ADJ, int LANES>
-__global__ void __launch_bounds__(kRotThreads, V == 8 ? 5 : V > 1 ? 4 : 1) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(kRotThreads, V > 1 ? 4 : 1) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   extern __shared__ __align__(16) float smem[];
   __shared__ i64 all_offs[kRotWarps][kRotMaxTile][4];  // token offsets of q, k, q_out, k_out
   const int row = a.slots * V, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -113,8 +113,16 @@ class Rendezvous:
         return bytes(self.store.get(key))
 
     def barrier(self) -> None:
-        """Host-side barrier (milliseconds; not for timed regions)."""
+        """Host-side barrier (milliseconds; not for timed regions).  Rank 0, whose process may serve the
+        store, returns when every other rank has read what it waited for: it may exit right away."""
         self.share(b"")
+        if self.world == 1:
+            return
+        if self.rank != 0:
+            self.store.set(f"twg/passed/{self._round}/{self.rank}", b"")
+        else:
+            for r in range(1, self.world):
+                self.store.get(f"twg/passed/{self._round}/{r}")
 
 
 # ---------------------------------------------------------------------------------------------
